@@ -73,6 +73,7 @@
 
 #include <hip/hip_runtime.h>
 #include <stdbool.h>
+#include <stddef.h>
 #include <stdint.h>
 
 #ifdef __cplusplus
@@ -409,6 +410,122 @@ bool flash_attn_rotary_apply(const void * const x, void * const out, const void 
                              const int64_t out_row_stride, const int64_t out_head_stride,
                              const int64_t cos_row_stride, const bool interleaved, const bool conj,
                              const bool is_bf16, hipStream_t stream);
+
+/* Per-head RMS norm of q and k with the rotary embedding in the same pass.  q, q_out: (batch, seqlen,
+ * num_heads, head_size), k, k_out: num_heads_k heads; ELEMENT strides {batch, row, head}, contiguous
+ * last dim, head_size <= 256; an output may be its input.  For each head's row x:
+ * z = weight * x / sqrt(mean(x^2) + eps), then the pairs of the first rotary_dim columns (the two
+ * halves, or (even, odd) columns when interleaved) become z1 cos - z2 sin, z1 sin + z2 cos; fp32
+ * arithmetic, one rounding.  q_weight, k_weight: (head_size), NULL for 1; cos, sin: (table_rows,
+ * rotary_dim / 2) with row stride cos_row_stride, both NULL (rotary_dim 0) for no rotation; positions:
+ * int32 (batch, seqlen) with stride positions_batch_stride, the table row of each token, NULL for
+ * 0 .. seqlen - 1.  A token whose position is outside the table gives NaN.  weight_fp32 / table_fp32:
+ * fp32 weights / tables, else the input dtype. */
+bool flash_attn_qk_norm_rotary(const void * const q, const void * const k, void * const q_out,
+                               void * const k_out, const void * const q_weight,
+                               const void * const k_weight, const void * const cos,
+                               const void * const sin, const int32_t * const positions,
+                               const int batch_size, const int seqlen, const int num_heads,
+                               const int num_heads_k, const int head_size, const int rotary_dim,
+                               const int table_rows, const float eps,
+                               const int64_t * const q_strides, const int64_t * const k_strides,
+                               const int64_t * const q_out_strides,
+                               const int64_t * const k_out_strides,
+                               const int64_t positions_batch_stride, const int64_t cos_row_stride,
+                               const bool weight_fp32, const bool table_fp32,
+                               const bool interleaved, const bool is_bf16, hipStream_t stream);
+
+/* Its backward: dq, dk from dq_out, dk_out and the forward's inputs; dq_weight, dk_weight (the weights'
+ * dtype, NULL when not wanted) are summed in fp32 in a fixed order through `workspace`, at least
+ * flash_attn_qk_norm_rotary_workspace(head_size) bytes (NULL without weight gradients). */
+bool flash_attn_qk_norm_rotary_bwd(const void * const dq_out, const void * const dk_out,
+                                   const void * const q, const void * const k, void * const dq,
+                                   void * const dk, const void * const q_weight,
+                                   const void * const k_weight, void * const dq_weight,
+                                   void * const dk_weight, const void * const cos,
+                                   const void * const sin, const int32_t * const positions,
+                                   void * const workspace, const int batch_size, const int seqlen,
+                                   const int num_heads, const int num_heads_k, const int head_size,
+                                   const int rotary_dim, const int table_rows, const float eps,
+                                   const int64_t * const dq_out_strides,
+                                   const int64_t * const dk_out_strides,
+                                   const int64_t * const q_strides, const int64_t * const k_strides,
+                                   const int64_t * const dq_strides,
+                                   const int64_t * const dk_strides,
+                                   const int64_t positions_batch_stride,
+                                   const int64_t cos_row_stride, const bool weight_fp32,
+                                   const bool table_fp32, const bool interleaved,
+                                   const bool is_bf16, hipStream_t stream);
+size_t flash_attn_qk_norm_rotary_workspace(int head_size);
+
+/* Key/value cache.  k_cache, v_cache: (batch, slots, num_heads_k, head_size), or with block_table pages
+ * (num_pages, page_size, num_heads_k, head_size); cache_strides = {sequence or page, row, head} in
+ * ELEMENTS, the same for both, multiples of 8 on 16-byte bases; block_table: int32, row stride
+ * block_table_stride, entry [i][j / page_size] is the page of key j of sequence i; page_size 0: none.
+ * `slots` is the number of keys a sequence has room for (with pages at most entries x page_size).
+ * cache_seqlens: int32 (batch), the keys each sequence holds.  head_size % 8 == 0, <= 256.
+ * No entry point reads or writes outside the cache whatever cache_seqlens and block_table hold.
+ *
+ * Attention of seqlen_q drafted tokens (1: plain decoding) that follow the cached keys at slots
+ * cache_seqlens[i] ...: row t sees every cached key and the drafted keys u with tree_mask[i][t][u] != 0
+ * (bytes, strides {batch, row}; NULL: u <= t).  k_new, v_new (NULL: the drafted keys are in the cache
+ * already) are also stored into those slots.  out (batch, seqlen_q, num_heads, head_size);
+ * softmax_lse (batch, num_heads, seqlen_q) fp32; rows that see no key give out = 0, LSE = +inf.
+ * attn_weight (fp32, optional): [i][kv head][key] += the sum over the rows of that kv head's query
+ * heads of exp(softmax_scale q.k - LSE), strides {batch, head}.  A sequence whose length leaves no
+ * room for the drafted tokens gives NaN and stores nothing; a page outside the cache gives NaN.
+ * strides arguments: {batch, row, head}.  workspace: flash_attn_kvcache_workspace(...) bytes. */
+bool flash_attn_kvcache(const void * const q, void * const k_cache, void * const v_cache,
+                        const void * const k_new, const void * const v_new, void * const out,
+                        float * const softmax_lse, float * const attn_weight,
+                        const int32_t * const cache_seqlens, const int32_t * const block_table,
+                        const uint8_t * const tree_mask, void * const workspace,
+                        const int batch_size, const int seqlen_q, const int slots,
+                        const int num_heads, const int num_heads_k, const int head_size,
+                        const int page_size, const int num_pages, const float softmax_scale,
+                        const int64_t * const q_strides, const int64_t * const cache_strides,
+                        const int64_t * const k_new_strides, const int64_t * const v_new_strides,
+                        const int64_t * const out_strides, const int64_t block_table_stride,
+                        const int64_t * const tree_mask_strides,
+                        const int64_t * const attn_weight_strides, const bool is_bf16,
+                        hipStream_t stream);
+size_t flash_attn_kvcache_workspace(int batch_size, int seqlen_q, int slots, int num_heads,
+                                    int num_heads_k, int head_size);
+
+/* Eviction in place.  Sequences with n > budget keys keep, for each kv head, the first `sink` keys, the
+ * last `recent` and of the others those of the largest attn_weight (equal: the lowest index), budget
+ * in all, moved to slots 0 .. budget - 1 in their order.  seqlens_out[i] = min(n, budget); kept
+ * (batch, num_heads_k, budget): the slot each kept key came from, -1 behind the last;
+ * attn_weight_out (strides {batch, head}, not attn_weight itself): the kept keys' weights, 0 in the
+ * slots behind them.  workspace: 4 batch num_heads_k bytes.  A sequence whose length is outside
+ * [0, slots] stays as it is; a key on a page outside the cache is not moved.  No page may belong to
+ * two sequences. */
+bool flash_attn_kvcache_evict(void * const k_cache, void * const v_cache,
+                              const int32_t * const cache_seqlens, const float * const attn_weight,
+                              const int32_t * const block_table, int32_t * const seqlens_out,
+                              float * const attn_weight_out, int32_t * const kept,
+                              void * const workspace, const int batch_size, const int slots,
+                              const int num_heads_k, const int head_size, const int page_size,
+                              const int num_pages, const int budget, const int sink,
+                              const int recent, const int64_t * const cache_strides,
+                              const int64_t block_table_stride,
+                              const int64_t * const attn_weight_strides,
+                              const int64_t * const attn_weight_out_strides, hipStream_t stream);
+
+/* Commit in place: of the seqlen_q drafted keys at slots cache_seqlens[i] ..., those with
+ * accepted[i][t] != 0 (bytes) move to the slots right behind the cached keys, in their order;
+ * seqlens_out[i] = cache_seqlens[i] + their number.  attn_weight (optional) moves along, 0 in the
+ * drafted slots behind.  A sequence whose length leaves no room for the drafted tokens stays as it is. */
+bool flash_attn_kvcache_commit(void * const k_cache, void * const v_cache,
+                               const int32_t * const cache_seqlens, const uint8_t * const accepted,
+                               const int32_t * const block_table, int32_t * const seqlens_out,
+                               float * const attn_weight, const int batch_size, const int seqlen_q,
+                               const int slots, const int num_heads_k, const int head_size,
+                               const int page_size, const int num_pages,
+                               const int64_t * const cache_strides,
+                               const int64_t block_table_stride,
+                               const int64_t accepted_batch_stride,
+                               const int64_t * const attn_weight_strides, hipStream_t stream);
 
 /* Tile sizes (block_m x block_n) of the forward / backward launchers for head_size. */
 void flash_attn_block_size(int head_size, int is_backward, int * block_m, int * block_n);

@@ -458,4 +458,239 @@ bool flash_attn_rotary_apply(const void* const x, void* const out, const void* c
   FA_END
 }
 
+// ---- norm + rotary, key/value cache (MI355X extensions; no reference counterpart) ----
+}  // extern "C"
+
+namespace {
+
+fa::QkNormTensor norm_tensor(const void* p, const int64_t* strides) {
+  FA_CHECK(p != nullptr && strides != nullptr);
+  return {p, strides[0], strides[1], strides[2]};
+}
+
+fa::QkNormParams norm_params(const void* q_weight, const void* k_weight, const void* cos, const void* sin,
+                             const int32_t* positions, int b, int seqlen, int h, int hk, int d, int rd, int table_rows,
+                             float eps, int64_t pos_batch, int64_t cs_row, bool weight_fp32, bool table_fp32,
+                             bool interleaved) {
+  check_device();
+  FA_CHECK(b >= 0 && seqlen >= 0 && h > 0 && hk > 0);
+  FA_CHECK(d > 0 && d <= 256);
+  FA_CHECK(rd >= 0 && rd <= d && rd % 2 == 0);
+  FA_CHECK((cos != nullptr) == (sin != nullptr) && (cos != nullptr) == (rd > 0));
+  if (rd > 0) FA_CHECK(table_rows > 0 && (positions != nullptr || table_rows >= seqlen));
+  FA_CHECK(eps >= 0.f);
+  FA_CHECK((int64_t)b * seqlen <= 0x7fffffff);
+  fa::QkNormParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.wq = q_weight; p.wk = k_weight;
+  p.cos = cos; p.sin = sin; p.positions = positions;
+  p.pos_batch = pos_batch; p.cs_row = cs_row;
+  p.b = b; p.seqlen = seqlen; p.h = h; p.hk = hk; p.d = d; p.rd = rd; p.table_rows = table_rows;
+  p.eps = eps; p.inv_d = 1.f / (float)d;
+  p.weight_f32 = weight_fp32; p.table_f32 = table_fp32; p.interleaved = interleaved;
+  return p;
+}
+
+fa::KvCache make_cache(void* k_cache, void* v_cache, const int32_t* lens, const int32_t* table, int64_t table_stride,
+                       const int64_t* strides, int b, int slots, int hk, int d, int page, int num_pages) {
+  check_device();
+  FA_CHECK(k_cache && v_cache && lens && strides);
+  FA_CHECK(b > 0 && slots > 0 && hk > 0);
+  FA_CHECK(d > 0 && d % 8 == 0 && d <= 256);
+  FA_CHECK((table != nullptr) == (page > 0));
+  if (table != nullptr) FA_CHECK(num_pages > 0);
+  FA_CHECK((uintptr_t)k_cache % 16 == 0 && (uintptr_t)v_cache % 16 == 0);
+  FA_CHECK(strides[0] % 8 == 0 && strides[1] % 8 == 0 && strides[2] % 8 == 0);
+  fa::KvCache c;
+  std::memset(&c, 0, sizeof(c));
+  c.k = k_cache; c.v = v_cache; c.table = table; c.lens = lens;
+  c.batch = strides[0]; c.row = strides[1]; c.head = strides[2];
+  c.table_row = table_stride;
+  c.b = b; c.hk = hk; c.d = d; c.slots = slots; c.page = page; c.num_pages = num_pages;
+  return c;
+}
+
+void attn_sizes(fa::KvAttnParams& p, int b, int sq, int slots, int h, int hk, int d) {
+  FA_CHECK(b > 0 && sq > 0 && h > 0 && hk > 0 && h % hk == 0);
+  FA_CHECK((int64_t)sq * (h / hk) <= (1 << 20) && slots <= 0x7fffff00);
+  p.c.b = b; p.c.hk = hk; p.c.d = d; p.c.slots = slots;
+  p.h = h; p.sq = sq; p.group = h / hk; p.rows = sq * p.group;
+  fa::kv_attn_plan(p);
+}
+
+// 16-byte vector access: the kernels read rows in chunks of 8 elements
+void check_vector(const void* ptr, const int64_t* strides) {
+  FA_CHECK(ptr != nullptr && strides != nullptr);
+  FA_CHECK((uintptr_t)ptr % 16 == 0);
+  FA_CHECK(strides[0] % 8 == 0 && strides[1] % 8 == 0 && strides[2] % 8 == 0);
+}
+
+}  // namespace
+
+extern "C" {
+
+bool flash_attn_qk_norm_rotary(const void* const q, const void* const k, void* const q_out, void* const k_out,
+                               const void* const q_weight, const void* const k_weight, const void* const cos,
+                               const void* const sin, const int32_t* const positions, const int batch_size,
+                               const int seqlen, const int num_heads, const int num_heads_k, const int head_size,
+                               const int rotary_dim, const int table_rows, const float eps,
+                               const int64_t* const q_strides, const int64_t* const k_strides,
+                               const int64_t* const q_out_strides, const int64_t* const k_out_strides,
+                               const int64_t positions_batch_stride, const int64_t cos_row_stride,
+                               const bool weight_fp32, const bool table_fp32, const bool interleaved,
+                               const bool is_bf16, hipStream_t stream) {
+  FA_BEGIN
+  fa::QkNormParams p = norm_params(q_weight, k_weight, cos, sin, positions, batch_size, seqlen, num_heads, num_heads_k,
+                                   head_size, rotary_dim, table_rows, eps, positions_batch_stride, cos_row_stride,
+                                   weight_fp32, table_fp32, interleaved);
+  p.q = norm_tensor(q, q_strides); p.k = norm_tensor(k, k_strides);
+  p.q_out = norm_tensor(q_out, q_out_strides); p.k_out = norm_tensor(k_out, k_out_strides);
+  fa::launch_qk_norm(p, false, is_bf16, stream);
+  return true;
+  FA_END
+}
+
+bool flash_attn_qk_norm_rotary_bwd(
+    const void* const dq_out, const void* const dk_out, const void* const q, const void* const k, void* const dq,
+    void* const dk, const void* const q_weight, const void* const k_weight, void* const dq_weight,
+    void* const dk_weight, const void* const cos, const void* const sin, const int32_t* const positions,
+    void* const workspace, const int batch_size, const int seqlen, const int num_heads, const int num_heads_k,
+    const int head_size, const int rotary_dim, const int table_rows, const float eps,
+    const int64_t* const dq_out_strides, const int64_t* const dk_out_strides, const int64_t* const q_strides,
+    const int64_t* const k_strides, const int64_t* const dq_strides, const int64_t* const dk_strides,
+    const int64_t positions_batch_stride, const int64_t cos_row_stride, const bool weight_fp32, const bool table_fp32,
+    const bool interleaved, const bool is_bf16, hipStream_t stream) {
+  FA_BEGIN
+  fa::QkNormParams p = norm_params(q_weight, k_weight, cos, sin, positions, batch_size, seqlen, num_heads, num_heads_k,
+                                   head_size, rotary_dim, table_rows, eps, positions_batch_stride, cos_row_stride,
+                                   weight_fp32, table_fp32, interleaved);
+  p.q = norm_tensor(q, q_strides); p.k = norm_tensor(k, k_strides);
+  p.q_grad = norm_tensor(dq_out, dq_out_strides); p.k_grad = norm_tensor(dk_out, dk_out_strides);
+  p.q_out = norm_tensor(dq, dq_strides); p.k_out = norm_tensor(dk, dk_strides);
+  p.dwq = dq_weight; p.dwk = dk_weight;
+  if (dq_weight != nullptr || dk_weight != nullptr) {
+    FA_CHECK(workspace != nullptr);
+    p.dw_part = static_cast<float*>(workspace);
+  }
+  fa::launch_qk_norm(p, true, is_bf16, stream);
+  return true;
+  FA_END
+}
+
+size_t flash_attn_qk_norm_rotary_workspace(int head_size) {
+  return head_size > 0 ? (size_t)fa::kQkNormMaxBlocks * head_size * sizeof(float) : 0;
+}
+
+bool flash_attn_kvcache(const void* const q, void* const k_cache, void* const v_cache, const void* const k_new,
+                        const void* const v_new, void* const out, float* const softmax_lse, float* const attn_weight,
+                        const int32_t* const cache_seqlens, const int32_t* const block_table,
+                        const uint8_t* const tree_mask, void* const workspace, const int batch_size,
+                        const int seqlen_q, const int slots, const int num_heads, const int num_heads_k,
+                        const int head_size, const int page_size, const int num_pages, const float softmax_scale,
+                        const int64_t* const q_strides, const int64_t* const cache_strides,
+                        const int64_t* const k_new_strides, const int64_t* const v_new_strides,
+                        const int64_t* const out_strides, const int64_t block_table_stride,
+                        const int64_t* const tree_mask_strides, const int64_t* const attn_weight_strides,
+                        const bool is_bf16, hipStream_t stream) {
+  FA_BEGIN
+  fa::KvAttnParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.c = make_cache(k_cache, v_cache, cache_seqlens, block_table, block_table_stride, cache_strides, batch_size, slots,
+                   num_heads_k, head_size, page_size, num_pages);
+  attn_sizes(p, batch_size, seqlen_q, slots, num_heads, num_heads_k, head_size);
+  FA_CHECK(softmax_lse != nullptr);
+  FA_CHECK(softmax_scale > 0.f && std::isfinite(softmax_scale));
+  FA_CHECK((k_new != nullptr) == (v_new != nullptr));
+  check_vector(q, q_strides);
+  check_vector(out, out_strides);
+  p.q = q; p.o = out; p.lse = softmax_lse;
+  p.q_batch = q_strides[0]; p.q_row = q_strides[1]; p.q_head = q_strides[2];
+  p.o_batch = out_strides[0]; p.o_row = out_strides[1]; p.o_head = out_strides[2];
+  if (k_new != nullptr) {
+    check_vector(k_new, k_new_strides);
+    check_vector(v_new, v_new_strides);
+    p.k_new = k_new; p.v_new = v_new;
+    p.kn_batch = k_new_strides[0]; p.kn_row = k_new_strides[1]; p.kn_head = k_new_strides[2];
+    p.vn_batch = v_new_strides[0]; p.vn_row = v_new_strides[1]; p.vn_head = v_new_strides[2];
+  }
+  if (tree_mask != nullptr) {
+    FA_CHECK(tree_mask_strides != nullptr);
+    p.mask = tree_mask; p.mask_batch = tree_mask_strides[0]; p.mask_row = tree_mask_strides[1];
+  }
+  if (attn_weight != nullptr) {
+    FA_CHECK(attn_weight_strides != nullptr);
+    p.weight = attn_weight; p.w_batch = attn_weight_strides[0]; p.w_head = attn_weight_strides[1];
+  }
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  if (fa::kv_attn_workspace(p) > 0) FA_CHECK(workspace != nullptr);
+  fa::launch_kv_attn(p, workspace, is_bf16, stream);
+  return true;
+  FA_END
+}
+
+size_t flash_attn_kvcache_workspace(int batch_size, int seqlen_q, int slots, int num_heads, int num_heads_k,
+                                    int head_size) {
+  try {
+    fa::KvAttnParams p;
+    std::memset(&p, 0, sizeof(p));
+    FA_CHECK(slots > 0 && head_size > 0);
+    attn_sizes(p, batch_size, seqlen_q, slots, num_heads, num_heads_k, head_size);
+    return fa::kv_attn_workspace(p);
+  } catch (const std::exception& e) {   // the call itself reports the sizes
+    set_error(e.what());
+    return 0;
+  }
+}
+
+bool flash_attn_kvcache_evict(void* const k_cache, void* const v_cache, const int32_t* const cache_seqlens,
+                              const float* const attn_weight, const int32_t* const block_table,
+                              int32_t* const seqlens_out, float* const attn_weight_out, int32_t* const kept,
+                              void* const workspace, const int batch_size, const int slots, const int num_heads_k,
+                              const int head_size, const int page_size, const int num_pages, const int budget,
+                              const int sink, const int recent, const int64_t* const cache_strides,
+                              const int64_t block_table_stride, const int64_t* const attn_weight_strides,
+                              const int64_t* const attn_weight_out_strides, hipStream_t stream) {
+  FA_BEGIN
+  fa::KvEvictParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.c = make_cache(k_cache, v_cache, cache_seqlens, block_table, block_table_stride, cache_strides, batch_size, slots,
+                   num_heads_k, head_size, page_size, num_pages);
+  FA_CHECK(attn_weight && seqlens_out && attn_weight_out && kept && workspace);
+  FA_CHECK(attn_weight_strides && attn_weight_out_strides && attn_weight != attn_weight_out);
+  FA_CHECK(budget > 0 && sink >= 0 && recent >= 0 && (int64_t)sink + recent <= budget);
+  FA_CHECK(batch_size <= 65535);
+  p.weight = attn_weight; p.w_batch = attn_weight_strides[0]; p.w_head = attn_weight_strides[1];
+  p.weight_out = attn_weight_out; p.wo_batch = attn_weight_out_strides[0]; p.wo_head = attn_weight_out_strides[1];
+  p.kept = kept; p.lens_out = seqlens_out; p.first = static_cast<int*>(workspace);
+  p.budget = budget; p.sink = sink; p.recent = recent;
+  fa::launch_kv_evict(p, stream);
+  return true;
+  FA_END
+}
+
+bool flash_attn_kvcache_commit(void* const k_cache, void* const v_cache, const int32_t* const cache_seqlens,
+                               const uint8_t* const accepted, const int32_t* const block_table,
+                               int32_t* const seqlens_out, float* const attn_weight, const int batch_size,
+                               const int seqlen_q, const int slots, const int num_heads_k, const int head_size,
+                               const int page_size, const int num_pages, const int64_t* const cache_strides,
+                               const int64_t block_table_stride, const int64_t accepted_batch_stride,
+                               const int64_t* const attn_weight_strides, hipStream_t stream) {
+  FA_BEGIN
+  fa::KvCommitParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.c = make_cache(k_cache, v_cache, cache_seqlens, block_table, block_table_stride, cache_strides, batch_size, slots,
+                   num_heads_k, head_size, page_size, num_pages);
+  FA_CHECK(accepted && seqlens_out);
+  FA_CHECK(seqlen_q > 0 && seqlen_q <= 8192);
+  p.accepted = accepted; p.acc_batch = accepted_batch_stride;
+  p.lens_out = seqlens_out; p.sq = seqlen_q;
+  if (attn_weight != nullptr) {
+    FA_CHECK(attn_weight_strides != nullptr);
+    p.weight = attn_weight; p.w_batch = attn_weight_strides[0]; p.w_head = attn_weight_strides[1];
+  }
+  fa::launch_kv_commit(p, stream);
+  return true;
+  FA_END
+}
+
 }  // extern "C"

@@ -149,6 +149,71 @@ struct RotaryParams {
   int64_t cs_row;
 };
 
+// Per-head RMS norm of q and k with the rotary embedding (fa_qknorm.hip): (b, seqlen, heads, d) tensors
+// with element strides and a contiguous last dim.  Forward: q, k -> q_out, k_out.  Backward: also the
+// output gradients q_grad, k_grad; q_out, k_out receive dq, dk; dwq, dwk (optional) the gains' gradients
+// through the fp32 partials dw_part, kQkNormMaxBlocks x d.
+constexpr int kQkNormMaxBlocks = 1024;
+struct QkNormTensor {
+  const void* ptr;
+  int64_t batch, row, head;
+};
+struct QkNormParams {
+  QkNormTensor q, k, q_out, k_out, q_grad, k_grad;
+  const void* wq; const void* wk;       // (d), or nullptr
+  void* dwq; void* dwk;
+  float* dw_part;
+  const void* cos; const void* sin;     // (table_rows, rd / 2), row stride cs_row, or nullptr (rd = 0)
+  const int* positions;                 // (b, seqlen) with batch stride pos_batch, or nullptr: 0 .. seqlen - 1
+  int64_t pos_batch, cs_row;
+  int b, seqlen, h, hk, d, rd, table_rows;
+  int blocks_q;                         // workgroups of q in the backward (set by the launcher)
+  float eps, inv_d;
+  bool weight_f32, table_f32, interleaved;
+};
+
+// Key/value cache (fa_kvcache.hip).  The cache is (b, slots, hk, d) (table == nullptr) or pages of
+// (num_pages, page, hk, d) with table (b, blocks) naming the page of each block of `page` keys; K and V
+// share their strides.  Sequence i holds lens[i] keys; sq drafted tokens follow at slots lens[i] ...
+struct KvCache {
+  void* k; void* v;
+  const int* table;
+  const int* lens;
+  int64_t batch, row, head;             // batch: of a sequence, or of a page
+  int64_t table_row;
+  int b, hk, d;
+  int slots;                            // keys a sequence has room for
+  int page, num_pages;                  // 0, 0 without a table
+};
+struct KvAttnParams {
+  KvCache c;
+  const void* q; void* o; float* lse;   // q, o: (b, sq, h, d); lse: (b, h, sq) fp32
+  const void* k_new; const void* v_new; // (b, sq, hk, d) or nullptr: the drafted keys are in the cache
+  const uint8_t* mask;                  // (b, sq, sq) bytes or nullptr: token i sees tokens 0 .. i
+  float* weight;                        // (b, hk, >= slots) fp32 or nullptr: += the keys' probabilities
+  float* part_o; float* part_lse;       // splits > 1: (b hk, splits, rows, d) and (b hk, splits, rows)
+  int64_t q_batch, q_row, q_head, o_batch, o_row, o_head;
+  int64_t kn_batch, kn_row, kn_head, vn_batch, vn_row, vn_head;
+  int64_t mask_batch, mask_row, w_batch, w_head;
+  int h, sq, group, rows;               // rows = sq * group
+  int m_tiles, splits;
+  float scale_log2;
+};
+struct KvEvictParams {
+  KvCache c;
+  const float* weight; float* weight_out; int64_t w_batch, w_head, wo_batch, wo_head;
+  int* kept; int* lens_out;             // (b, hk, budget), (b)
+  int* first;                           // (b, hk): the first place whose key moves
+  int budget, sink, recent;
+};
+struct KvCommitParams {
+  KvCache c;
+  const uint8_t* accepted; int64_t acc_batch;   // (b, sq) bytes
+  float* weight; int64_t w_batch, w_head;       // optional, compacted with the keys
+  int* lens_out;
+  int sq;
+};
+
 // Q' = bf16/f16(c Q) in the compact layout (b | padded rows, seqlen_q, h, d): rows at the sequence
 // offsets the kernels use (batch b at b seqlen_q h d; varlen at cu_seqlens_q[b] h d), so the
 // consumers address it with q_batch = seqlen_q h d, q_row = h d, q_head = d (fa_bwd.hip
@@ -191,6 +256,13 @@ bool dq_asm_applicable(const BwdParams& p, bool fused);                         
 void launch_bwd_dq_asm(const BwdParams& p, bool is_bf16, hipStream_t stream);
 void launch_reduced_scores(const ReducedParams& p, bool is_bf16, hipStream_t stream);
 void launch_rotary(const RotaryParams& p, bool interleaved, bool conj, bool is_bf16, hipStream_t stream);
+void launch_qk_norm(QkNormParams p, bool backward, bool is_bf16, hipStream_t stream);
+// fa_kvcache.hip: the split of a call (rows tiles, key splits) follows from its sizes alone
+void kv_attn_plan(KvAttnParams& p);
+size_t kv_attn_workspace(const KvAttnParams& p);   // bytes of part_o + part_lse
+void launch_kv_attn(KvAttnParams p, void* workspace, bool is_bf16, hipStream_t stream);
+void launch_kv_evict(const KvEvictParams& p, hipStream_t stream);
+void launch_kv_commit(const KvCommitParams& p, hipStream_t stream);
 
 // Tile sizes the launchers use for a given head dim (reported by _get_block_size in Python).
 void fwd_block_size(int d, int* block_m, int* block_n);

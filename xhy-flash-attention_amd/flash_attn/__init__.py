@@ -7,3 +7,6 @@ from flash_attn.flash_attn_interface import flash_attn_qkvpacked_func
 from flash_attn.flash_attn_interface import flash_attn_varlen_qkvpacked_func
 from flash_attn.flash_attn_interface import flash_attn_varlen_kvpacked_func
 from flash_attn.flash_attn_interface import flash_attn_varlen_func
+from flash_attn.kvcache_interface import flash_attn_kvcache_commit_
+from flash_attn.kvcache_interface import flash_attn_kvcache_evict_
+from flash_attn.kvcache_interface import flash_attn_kvcache_func
