@@ -45,7 +45,8 @@ REFUSED = [
     (dict(v=torch.zeros(2, 3, 2, 64, dtype=torch.float16)), "the cache's dtype"),
     (dict(tree_mask=torch.ones(3, 3)), "tree_mask must be bool"),
     (dict(tree_mask=torch.ones(3, 4, dtype=torch.bool)), "tree_mask must be bool"),
-    (dict(attn_weight=torch.zeros(2, 2, 49)), "attn_weight must be fp32"),
+    (dict(attn_weight=torch.zeros(2, 3, 50)), "attn_weight must be fp32"),
+    (dict(attn_weight=torch.zeros(2, 2, 2)), "more drafted tokens"),
     (dict(attn_weight=torch.zeros(2, 2, 50, dtype=BF)), "attn_weight must be fp32"),
     (dict(softmax_scale=0.0), "positive and finite"),
     (dict(softmax_scale=-1.0), "positive and finite"),

@@ -77,9 +77,11 @@ def _check_device(*tensors):
 
 
 def _check_weight(w, b, hk, slots):
-    _ext._check(w.dtype == torch.float32 and w.dim() == 3 and tuple(w.shape[:2]) == (b, hk) and w.shape[2] >= slots,
+    """Returns the slots that a call with these weights has room for."""
+    _ext._check(w.dtype == torch.float32 and w.dim() == 3 and tuple(w.shape[:2]) == (b, hk) and w.shape[2] > 0,
                 "kvcache: attn_weight must be fp32 (batch, nheads_k, slots)")
     _ext._check(w.stride(2) == 1, "kvcache: attn_weight must have a contiguous last dimension")
+    return min(slots, w.shape[2])
 
 
 def _flag_bytes(m, shape, name):
@@ -111,7 +113,8 @@ def flash_attn_kvcache_func(q, k_cache, v_cache, cache_seqlens, k=None, v=None, 
             seen.  A drafted token that no row sees may hold anything.
         softmax_scale: default 1 / sqrt(headdim).
         attn_weight: fp32 (batch, nheads_k, slots), optional: every key's entry grows by the sum of its
-            probabilities over the rows of the query heads that share the kv head.
+            probabilities over the rows of the query heads that share the kv head.  With fewer columns
+            than the cache has slots, sequences have room for as many keys (in the other calls too).
         return_softmax_lse: also return the log-sum-exp of the scaled scores, fp32 (batch, nheads, seqlen_q).
     cache_seqlens is not changed (flash_attn_kvcache_commit_ gives the new lengths).  A row that sees
     no key gives 0 and +inf.  A sequence whose length leaves no room for the drafted tokens, or that
@@ -123,6 +126,8 @@ def flash_attn_kvcache_func(q, k_cache, v_cache, cache_seqlens, k=None, v=None, 
     check(q.dim() == 4 and q.shape[0] == b and q.shape[3] == d,
           "kvcache: q must have shape (batch, seqlen_q, nheads, headdim)")
     sq, h = q.shape[1:3]
+    if attn_weight is not None:
+        slots = _check_weight(attn_weight, b, hk, slots)
     check(sq > 0, "kvcache: at least one drafted token")
     check(h > 0 and h % hk == 0, "Number of heads in key/value must divide number of heads in query")
     check(sq <= slots, "kvcache: more drafted tokens than slots")
@@ -137,8 +142,6 @@ def flash_attn_kvcache_func(q, k_cache, v_cache, cache_seqlens, k=None, v=None, 
     if tree_mask is not None:
         tree_mask = _flag_bytes(tree_mask, ((sq, sq), (b, sq, sq)), "tree_mask")
         mstr = _ints(tree_mask.stride(0) if tree_mask.dim() == 3 else 0, tree_mask.stride(-2))
-    if attn_weight is not None:
-        _check_weight(attn_weight, b, hk, slots)
     scale = d ** -0.5 if softmax_scale is None else float(softmax_scale)
     check(0.0 < scale < float("inf"), "kvcache: softmax_scale must be positive and finite")
     _check_device(k_cache, v_cache, cache_seqlens, block_table, q, k, v, tree_mask, attn_weight)
@@ -176,11 +179,11 @@ def flash_attn_kvcache_commit_(k_cache, v_cache, cache_seqlens, accepted, block_
     hk, d = k_cache.shape[2:]
     _ext._check(accepted.dim() == 2 and accepted.shape[0] == b, "kvcache: accepted must be bool (batch, seqlen_q)")
     sq = accepted.shape[1]
+    if attn_weight is not None:
+        slots = _check_weight(attn_weight, b, hk, slots)
     _ext._check(0 < sq <= 8192 and sq <= slots, "kvcache: between 1 and min(8192, slots) drafted tokens")
     accepted = _flag_bytes(accepted, ((b, sq),), "accepted")
     _check_no_grad(k_cache, v_cache)
-    if attn_weight is not None:
-        _check_weight(attn_weight, b, hk, slots)
     _check_device(k_cache, v_cache, cache_seqlens, block_table, accepted, attn_weight)
     ptr = _ext._ptr
     with _ext._device_guard(k_cache.device):
@@ -213,7 +216,7 @@ def flash_attn_kvcache_evict_(k_cache, v_cache, cache_seqlens, attn_weight, budg
     _ext._check(0 < budget < 2 ** 31 and sink >= 0 and recent >= 0 and sink + recent <= budget,
                 "kvcache: budget must be positive and at least sink + recent")
     _ext._check(b <= 65535, "kvcache: batch size must be at most 65535")
-    _check_weight(attn_weight, b, hk, slots)
+    slots = _check_weight(attn_weight, b, hk, slots)
     _check_no_grad(k_cache, v_cache, attn_weight)
     _check_device(k_cache, v_cache, cache_seqlens, block_table, attn_weight)
     ptr = _ext._ptr
