@@ -474,7 +474,8 @@ size_t flash_attn_qk_norm_rotary_workspace(int head_size);
  * attn_weight (fp32, optional): [i][kv head][key] += the sum over the rows of that kv head's query
  * heads of exp(softmax_scale q.k - LSE), strides {batch, head}.  A sequence whose length leaves no
  * room for the drafted tokens gives NaN and stores nothing; a page outside the cache gives NaN.
- * strides arguments: {batch, row, head}.  workspace: flash_attn_kvcache_workspace(...) bytes. */
+ * strides arguments: {batch, row, head}.  workspace: flash_attn_kvcache_workspace(...) bytes, 16-byte
+ * aligned (attn_weight: whether the call has one). */
 bool flash_attn_kvcache(const void * const q, void * const k_cache, void * const v_cache,
                         const void * const k_new, const void * const v_new, void * const out,
                         float * const softmax_lse, float * const attn_weight,
@@ -490,7 +491,7 @@ bool flash_attn_kvcache(const void * const q, void * const k_cache, void * const
                         const int64_t * const attn_weight_strides, const bool is_bf16,
                         hipStream_t stream);
 size_t flash_attn_kvcache_workspace(int batch_size, int seqlen_q, int slots, int num_heads,
-                                    int num_heads_k, int head_size);
+                                    int num_heads_k, int head_size, bool attn_weight);
 
 /* Eviction in place.  Sequences with n > budget keys keep, for each kv head, the first `sink` keys, the
  * last `recent` and of the others those of the largest attn_weight (equal: the lowest index), budget

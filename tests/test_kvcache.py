@@ -112,11 +112,11 @@ def test_c_abi_refuses_without_touching_memory():
     assert lib.flash_attn_error()
     assert lib.flash_attn_kvcache_evict(*[None] * 9, 1, 1, 1, 8, 0, 0, 0, 0, 0, z, 0, z, z, None) is False
     assert lib.flash_attn_kvcache_commit(*[None] * 7, 1, 1, 1, 1, 8, 0, 0, z, 0, 0, z, None) is False
-    assert lib.flash_attn_kvcache_workspace(1, 1, 0, 1, 1, 64) == 0
-    assert lib.flash_attn_kvcache_workspace(1, 1, 100, 3, 2, 64) == 0
+    assert lib.flash_attn_kvcache_workspace(1, 1, 0, 1, 1, 64, False) == 0
+    assert lib.flash_attn_kvcache_workspace(1, 1, 100, 3, 2, 64, False) == 0
     # small caches need no split and no workspace; long ones one partial row per split, fp32
-    assert lib.flash_attn_kvcache_workspace(1, 1, 100, 2, 2, 64) == 0
-    size = lib.flash_attn_kvcache_workspace(1, 2, 65536, 4, 2, 128)
+    assert lib.flash_attn_kvcache_workspace(1, 1, 100, 2, 2, 64, False) == 0
+    size = lib.flash_attn_kvcache_workspace(1, 2, 65536, 4, 2, 128, False)
     assert size > 0 and size % (2 * 4 * 129 * 4) == 0
 
 

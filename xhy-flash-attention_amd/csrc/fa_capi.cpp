@@ -513,14 +513,17 @@ fa::KvCache make_cache(void* k_cache, void* v_cache, const int32_t* lens, const 
 void attn_sizes(fa::KvAttnParams& p, int b, int sq, int slots, int h, int hk, int d) {
   FA_CHECK(b > 0 && sq > 0 && h > 0 && hk > 0 && h % hk == 0);
   FA_CHECK((int64_t)sq * (h / hk) <= (1 << 20) && slots <= 0x7fffff00);
+  FA_CHECK(d > 0 && d <= 256);
   p.c.b = b; p.c.hk = hk; p.c.d = d; p.c.slots = slots;
   p.h = h; p.sq = sq; p.group = h / hk; p.rows = sq * p.group;
   fa::kv_attn_plan(p);
 }
 
-// 16-byte vector access: the kernels read rows in chunks of 8 elements
-void check_vector(const void* ptr, const int64_t* strides) {
+// 16-byte vector access: the kernels read rows in chunks of 8 elements, those of a sequence's kv head at
+// byte offsets of 31 bits
+void check_vector(const void* ptr, const int64_t* strides, int64_t rows, int64_t heads) {
   FA_CHECK(ptr != nullptr && strides != nullptr);
+  FA_CHECK(strides[1] >= 0 && strides[2] >= 0 && rows * strides[1] + heads * strides[2] < (1 << 29));
   FA_CHECK((uintptr_t)ptr % 16 == 0);
   FA_CHECK(strides[0] % 8 == 0 && strides[1] % 8 == 0 && strides[2] % 8 == 0);
 }
@@ -601,20 +604,21 @@ bool flash_attn_kvcache(const void* const q, void* const k_cache, void* const v_
   FA_CHECK(softmax_lse != nullptr);
   FA_CHECK(softmax_scale > 0.f && std::isfinite(softmax_scale));
   FA_CHECK((k_new != nullptr) == (v_new != nullptr));
-  check_vector(q, q_strides);
-  check_vector(out, out_strides);
+  check_vector(q, q_strides, seqlen_q, p.group);
+  check_vector(out, out_strides, seqlen_q, p.group);
   p.q = q; p.o = out; p.lse = softmax_lse;
   p.q_batch = q_strides[0]; p.q_row = q_strides[1]; p.q_head = q_strides[2];
   p.o_batch = out_strides[0]; p.o_row = out_strides[1]; p.o_head = out_strides[2];
   if (k_new != nullptr) {
-    check_vector(k_new, k_new_strides);
-    check_vector(v_new, v_new_strides);
+    check_vector(k_new, k_new_strides, seqlen_q, 0);
+    check_vector(v_new, v_new_strides, seqlen_q, 0);
     p.k_new = k_new; p.v_new = v_new;
     p.kn_batch = k_new_strides[0]; p.kn_row = k_new_strides[1]; p.kn_head = k_new_strides[2];
     p.vn_batch = v_new_strides[0]; p.vn_row = v_new_strides[1]; p.vn_head = v_new_strides[2];
   }
   if (tree_mask != nullptr) {
     FA_CHECK(tree_mask_strides != nullptr);
+    FA_CHECK(tree_mask_strides[1] >= 0 && seqlen_q * tree_mask_strides[1] + seqlen_q < (1 << 30));
     p.mask = tree_mask; p.mask_batch = tree_mask_strides[0]; p.mask_row = tree_mask_strides[1];
   }
   if (attn_weight != nullptr) {
@@ -629,11 +633,14 @@ bool flash_attn_kvcache(const void* const q, void* const k_cache, void* const v_
 }
 
 size_t flash_attn_kvcache_workspace(int batch_size, int seqlen_q, int slots, int num_heads, int num_heads_k,
-                                    int head_size) {
+                                    int head_size, bool attn_weight) {
   try {
     fa::KvAttnParams p;
     std::memset(&p, 0, sizeof(p));
-    FA_CHECK(slots > 0 && head_size > 0);
+    float unused;
+    p.weight = attn_weight ? &unused : nullptr;
+    FA_CHECK(slots > 0);
+    p.c.row = head_size;   // (strides do not matter here)
     attn_sizes(p, batch_size, seqlen_q, slots, num_heads, num_heads_k, head_size);
     return fa::kv_attn_workspace(p);
   } catch (const std::exception& e) {   // the call itself reports the sizes

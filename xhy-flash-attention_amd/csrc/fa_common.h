@@ -218,6 +218,10 @@ __device__ inline float half_swap_sum(float x) {
 __device__ inline float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ inline float fast_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
 __device__ inline int wave_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ inline int64_t uniform64(int64_t x) {
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)x), hi = __builtin_amdgcn_readfirstlane((unsigned)(x >> 32));
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
 template <typename T> __device__ inline const T* uniform_ptr(const T* p) {
   const unsigned long long a = (unsigned long long)p;
   const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)a), hi = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32));

@@ -191,12 +191,14 @@ struct KvAttnParams {
   const void* k_new; const void* v_new; // (b, sq, hk, d) or nullptr: the drafted keys are in the cache
   const uint8_t* mask;                  // (b, sq, sq) bytes or nullptr: token i sees tokens 0 .. i
   float* weight;                        // (b, hk, >= slots) fp32 or nullptr: += the keys' probabilities
-  float* part_o; float* part_lse;       // splits > 1: (b hk, splits, rows, d) and (b hk, splits, rows)
+  float* part_o; float* part_lse;       // (shares, m_tiles, hk, 2, tile_rows, d) and (.., tile_rows)
+  float* scores; int64_t score_pitch;   // (b hk, rows, score_pitch), log2 units: stored for `weight`, or nullptr
   int64_t q_batch, q_row, q_head, o_batch, o_row, o_head;
   int64_t kn_batch, kn_row, kn_head, vn_batch, vn_row, vn_head;
   int64_t mask_batch, mask_row, w_batch, w_head;
   int h, sq, group, rows;               // rows = sq * group
-  int m_tiles, splits;
+  int m_tiles, tile_rows, shares;       // row tiles, rows of one, shares of the keys (kv_attn_plan)
+  bool even;                            // a wave's 32 keys are evenly strided
   float scale_log2;
 };
 struct KvEvictParams {
@@ -257,9 +259,9 @@ void launch_bwd_dq_asm(const BwdParams& p, bool is_bf16, hipStream_t stream);
 void launch_reduced_scores(const ReducedParams& p, bool is_bf16, hipStream_t stream);
 void launch_rotary(const RotaryParams& p, bool interleaved, bool conj, bool is_bf16, hipStream_t stream);
 void launch_qk_norm(QkNormParams p, bool backward, bool is_bf16, hipStream_t stream);
-// fa_kvcache.hip: the split of a call (rows tiles, key splits) follows from its sizes alone
+// fa_kvcache.hip: row tiles and workgroups follow from the call's sizes alone
 void kv_attn_plan(KvAttnParams& p);
-size_t kv_attn_workspace(const KvAttnParams& p);   // bytes of part_o + part_lse
+size_t kv_attn_workspace(const KvAttnParams& p);   // bytes of part_o, part_lse and scores
 void launch_kv_attn(KvAttnParams p, void* workspace, bool is_bf16, hipStream_t stream);
 void launch_kv_evict(const KvEvictParams& p, hipStream_t stream);
 void launch_kv_commit(const KvCommitParams& p, hipStream_t stream);

@@ -25,7 +25,7 @@ _lib = _ext._lib
 _P, _I, _I64, _F, _B = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_bool
 _lib.flash_attn_kvcache.argtypes = [_P] * 12 + [_I] * 8 + [_F] + [_P] * 5 + [_I64] + [_P] * 2 + [_B, _P]
 _lib.flash_attn_kvcache.restype = _B
-_lib.flash_attn_kvcache_workspace.argtypes = [_I] * 6
+_lib.flash_attn_kvcache_workspace.argtypes = [_I] * 6 + [_B]
 _lib.flash_attn_kvcache_workspace.restype = ctypes.c_size_t
 _lib.flash_attn_kvcache_evict.argtypes = [_P] * 9 + [_I] * 9 + [_P, _I64, _P, _P, _P]
 _lib.flash_attn_kvcache_evict.restype = _B
@@ -152,7 +152,7 @@ def flash_attn_kvcache_func(q, k_cache, v_cache, cache_seqlens, k=None, v=None, 
     with _ext._device_guard(q.device):
         out = torch.empty((b, sq, h, d), dtype=q.dtype, device=q.device)
         lse = torch.empty((b, h, sq), dtype=torch.float32, device=q.device)
-        size = _lib.flash_attn_kvcache_workspace(b, sq, slots, h, hk, d)
+        size = _lib.flash_attn_kvcache_workspace(b, sq, slots, h, hk, d, attn_weight is not None)
         work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
         none = _ints(0, 0, 0)
         ok = _lib.flash_attn_kvcache(
