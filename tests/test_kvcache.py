@@ -1,5 +1,6 @@
 """CPU checks of the key/value cache and norm + rotary entry points: what they refuse, and the cache
 addressing the kernels share (csrc/fa_kvcache.h), compiled for the host."""
+import ctypes
 import os
 import shutil
 import subprocess
@@ -105,19 +106,30 @@ def test_norm_rotary_refuses():
 def test_c_abi_refuses_without_touching_memory():
     """Sizes outside the contract come back as false with a message (on a GPU box the device check passes
     and the sizes are refused; here the device is), and the workspace query as 0."""
-    import flash_attn.kvcache_interface as m
-    lib, ints = m._lib, m._ints
-    z = ints(0, 0, 0)
-    assert lib.flash_attn_kvcache(*[None] * 12, 1, 1, 1, 1, 1, 60, 0, 0, 1.0, z, z, z, z, z, 0, z, z, True, None) is False
-    assert lib.flash_attn_error()
-    assert lib.flash_attn_kvcache_evict(*[None] * 9, 1, 1, 1, 8, 0, 0, 0, 0, 0, z, 0, z, z, None) is False
-    assert lib.flash_attn_kvcache_commit(*[None] * 7, 1, 1, 1, 1, 8, 0, 0, z, 0, 0, z, None) is False
-    assert lib.flash_attn_kvcache_workspace(1, 1, 0, 1, 1, 64, False) == 0
-    assert lib.flash_attn_kvcache_workspace(1, 1, 100, 3, 2, 64, False) == 0
-    # small caches need no split and no workspace; long ones one partial row per split, fp32
-    assert lib.flash_attn_kvcache_workspace(1, 1, 100, 2, 2, 64, False) == 0
-    size = lib.flash_attn_kvcache_workspace(1, 2, 65536, 4, 2, 128, False)
+    import flash_attn_2_cuda as m
+    lib = m._lib
+    P, I, L, F, B = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_bool
+    z = (L * 3)(0, 0, 0)
+    for name, kinds, args in (
+            ("flash_attn_kvcache", [P] * 12 + [I] * 8 + [F] + [P] * 5 + [L] + [P] * 2 + [B, P],
+             [None] * 12 + [1, 1, 1, 1, 1, 60, 0, 0, 1.0, z, z, z, z, z, 0, z, z, True, None]),
+            ("flash_attn_kvcache_evict", [P] * 9 + [I] * 9 + [P, L, P, P, P],
+             [None] * 9 + [1, 1, 1, 8, 0, 0, 0, 0, 0, z, 0, z, z, None]),
+            ("flash_attn_kvcache_commit", [P] * 7 + [I] * 7 + [P, L, L, P, P],
+             [None] * 7 + [1, 1, 1, 1, 8, 0, 0, z, 0, 0, z, None])):
+        f = getattr(lib, name)
+        f.argtypes, f.restype = kinds, B
+        assert f(*args) is False, name
+        assert lib.flash_attn_error()
+    w = lib.flash_attn_kvcache_workspace
+    w.argtypes, w.restype = [I] * 6 + [B], ctypes.c_size_t
+    assert w(1, 1, 0, 1, 1, 64, False) == 0
+    assert w(1, 1, 100, 3, 2, 64, False) == 0
+    # small caches are never cut and need no workspace; long ones hold fp32 rows and their LSE
+    assert w(1, 1, 100, 2, 2, 64, False) == 0
+    size = w(1, 2, 65536, 4, 2, 128, False)
     assert size > 0 and size % (2 * 4 * 129 * 4) == 0
+    assert w(1, 2, 65536, 4, 2, 128, True) == size + 2 * 4 * 65536 * 4
 
 
 HOST = r"""

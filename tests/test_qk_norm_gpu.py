@@ -125,6 +125,33 @@ def test_gradient_against_differences():
             assert abs(float((grads[2 + i].double() * dwv).sum()) - nw) <= tw
 
 
+def test_gradients_of_some_inputs_and_twice():
+    """Each subset of weights and leaves gives the full call's gradients; a second differentiation raises."""
+    q, k = (t.contiguous() for t in _make(1, 12, 4, 2, 64, torch.bfloat16))
+    w = [(1 + 0.2 * torch.randn(64, device=DEV)) for _ in range(2)]
+    cos, sin = _table(12, 64, torch.float32)
+    g = [torch.randn_like(q), torch.randn_like(k)]
+
+    def run(need, weights):
+        leaves = [t.clone().requires_grad_(n) for t, n in zip((q, k, *w), need)]
+        ww = [leaves[2 + i] if weights[i] else None for i in range(2)]
+        out = _func()(leaves[0], leaves[1], *ww, cos, sin)
+        torch.autograd.backward(out, g)
+        return [t.grad for t in leaves]
+
+    full = run((True,) * 4, (True, True))
+    for need in ((True, False, False, False), (False, False, False, True), (False, True, True, False)):
+        for a, b, n in zip(run(need, (True, True)), full, need):
+            assert (torch.equal(a, b) if n else a is None)
+    only_k = run((False, False, False, True), (False, True))
+    assert torch.equal(only_k[3], full[3]) and only_k[2] is None
+    leaf = q.clone().requires_grad_()
+    out = _func()(leaf, k, w[0], None, cos, sin)[0]
+    grad, = torch.autograd.grad(out.sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        grad.sum().backward()
+
+
 @pytest.mark.parametrize("d,rd", [(128, 128), (40, 22)])
 def test_forms_agree(d, rd):
     """No weights, one weight, no batch dimension, in place, positions 0 .. s-1: one result."""

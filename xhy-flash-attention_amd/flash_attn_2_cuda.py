@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import importlib.util
 import os
 
 import torch
@@ -53,6 +54,26 @@ _lib.flash_attn_block_size.argtypes = [_I, _I, ctypes.POINTER(_I), ctypes.POINTE
 _lib.flash_attn_block_size.restype = None
 
 _INT_MAX = 2 ** 31 - 1
+
+_HOST = None
+
+
+def host_module():
+    """``_flash_attn_host`` (csrc/fa_host.cpp), its entry points bound to the library loaded above."""
+    global _HOST
+    if _HOST is None:
+        path = os.path.join(_HERE, "_flash_attn_host.so")
+        if not os.path.exists(path):
+            raise ImportError(f"flash_attn_2_cuda: {path} is missing; build it with `make -C xhy-flash-attention_amd/csrc`")
+        spec = importlib.util.spec_from_file_location("_flash_attn_host", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind({name: ctypes.cast(getattr(_lib, name), ctypes.c_void_p).value for name in (
+            "flash_attn_qk_norm_rotary", "flash_attn_qk_norm_rotary_bwd", "flash_attn_qk_norm_rotary_workspace",
+            "flash_attn_kvcache", "flash_attn_kvcache_workspace", "flash_attn_kvcache_evict",
+            "flash_attn_kvcache_commit", "flash_attn_error")})
+        _HOST = module
+    return _HOST
 
 
 def block_size(head_dim: int, is_backward: bool = False):
