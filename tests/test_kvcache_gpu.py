@@ -271,7 +271,7 @@ def test_offsets_past_32_bits():
 @pytest.mark.parametrize("hk,d,lens,budget,sink,recent", [
     (2, 64, [100, 40, 41, 0], 40, 4, 10), (1, 128, [5000], 1200, 0, 0), (3, 8, [65, 300], 64, 0, 64),
     (2, 256, [700, 699], 130, 100, 30), (1, 40, [33], 1, 0, 0), (1, 40, [33], 1, 1, 0), (4, 96, [2500, 9], 2499, 7, 11),
-    (2, 128, [1500, 20], 3000, 1, 1)])
+    (2, 128, [1500, 20], 3000, 1, 1), (2, 8, [20000, 9000], 8888, 5, 100), (1, 16, [70000], 30000, 0, 1)])
 def test_evict(hk, d, lens, budget, sink, recent, page):
     from flash_attn import flash_attn_kvcache_evict_
     b = len(lens)

@@ -4,12 +4,12 @@
 // Eviction, for each (sequence, kv head) of n > budget keys with weights w: keep the first `sink` keys,
 // the last `recent`, and of the others the budget - sink - recent with the largest w (equal weights:
 // the lowest index); the kept keys move to places 0 .. budget - 1 in their order.  Two kernels:
-//   * select: one workgroup a (sequence, kv head).  The smallest kept weight is found by a radix
-//     select over order-preserving 32-bit images of the weights, 11 + 11 + 10 bits from the top, each
-//     pass a histogram in LDS of the keys that agree with the prefix found so far (the weights are
-//     re-read from L2: 4 bytes a key against the 4 d of its K and V).  One more pass counts, per wave
-//     over consecutive keys, those above and those equal; their prefix sums give every kept key its
-//     place without atomics, so the result is a function of the weights alone;
+//   * select: one workgroup a (sequence, kv head), which holds up to 32k weights in registers.  The
+//     smallest kept weight is found by a radix select over order-preserving 32-bit images of the weights,
+//     8 + 12 + 12 bits from the top, each pass a histogram in LDS of the keys that agree with the prefix
+//     found so far.  Weights crowd in a few exponents, so the first histogram has a copy for every two
+//     lanes.  One more pass counts, per wave over consecutive keys, those above and those equal;
+//     their prefix sums give every kept key its place, so the result is a function of the weights alone;
 //   * move: place i receives key kept[i] >= i.  A workgroup owns all rows of a 64-byte column slice of K
 //     or V of one (sequence, kv head) and walks the places upwards in chunks: the chunk's rows are in
 //     registers in every thread (barrier) before any of its places is written, and places below
@@ -25,6 +25,7 @@
 namespace fa {
 
 static constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
+static constexpr int kSelCopies = 32, kSelPitch = 257;   // histograms of the first pass, by lane (see below)
 static constexpr int kMoveThreads = 512;
 
 // 32-bit image of a weight: unsigned order = numeric order, NaN above +inf, -0 = +0
@@ -37,7 +38,10 @@ __device__ inline unsigned ordered(float x) {
 __device__ inline int wave_count(bool x) { return __popcll(__ballot(x)); }
 __device__ inline int lanes_below(bool x, int lane) { return __popcll(__ballot(x) & ((1ull << lane) - 1)); }
 
+// BATCH: keys a thread holds
+template <int BATCH>
 __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const KvEvictParams p) {
+  constexpr int CHUNK = kSelThreads * BATCH;
   const KvCache& c = p.c;
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_uniform(tid >> 6);
   const int kvh = blockIdx.x, bidb = blockIdx.y;
@@ -56,81 +60,138 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const KvEvictPar
     return;
   }
 
-  __shared__ int hist[2048];
-  __shared__ int wave_sum[kSelWaves], wave_sum2[kSelWaves];
+  __shared__ int hist[kSelCopies * kSelPitch];     // pass 0: copies of 256 bins; then one of 4096
+  __shared__ int wave_sum[2][kSelWaves], wave_sum2[2][kSelWaves];
   __shared__ int s_digit, s_need, s_first;
   const int lo = p.sink, hi = n - p.recent;       // the keys that compete
   int need = p.budget - p.sink - p.recent;        // how many of them stay
   unsigned prefix = 0;
   int shift = 32;
   if (tid == 0) s_first = n;
+  // The weights go by in chunks of consecutive keys, a wave 64 `used` of a chunk, all on their way at
+  // once; a head of one chunk keeps them in registers over all passes.
+  float x[BATCH];
+  unsigned image[BATCH];
+  int held = -1;
+  auto at = [&](int c0, int used, int u) { return c0 + (wave * used + u) * 64 + lane; };
+  auto competes = [&](int i) { return (unsigned)(i - lo) < (unsigned)(hi - lo); };   // (hi > lo: n > budget)
+  auto fetch = [&](int c0) {
+    const int used = min(BATCH, (n - c0 + kSelThreads - 1) / kSelThreads);
+    if (held != c0) {
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u)
+        if (u < used) x[u] = w[min(at(c0, used, u), n - 1)];
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u)
+        if (u < used) image[u] = ordered(x[u]);
+      held = c0;
+    }
+    return used;
+  };
 #pragma unroll 1
   for (int pass = 0; pass < 3 && need > 0; ++pass) {
-    const int bits = pass < 2 ? 11 : 10;
-    for (int i = tid; i < 2048; i += kSelThreads) hist[i] = 0;
+    const int bits = pass == 0 ? 8 : 12;
+    for (int i = tid; i < kSelCopies * kSelPitch; i += kSelThreads) hist[i] = 0;
     __syncthreads();
     const int top = shift;
     shift -= bits;
-    for (int i = lo + tid; i < hi; i += kSelThreads) {
-      const unsigned u = ordered(w[i]);
-      if (pass == 0 || (u >> top) == prefix) atomicAdd(&hist[(u >> shift) & ((1u << bits) - 1)], 1);
+    for (int c0 = 0; c0 < n; c0 += CHUNK) {
+      const int used = fetch(c0);
+      if (pass == 0) {
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u)
+          if (u < used && competes(at(c0, used, u)))
+            atomicAdd(&hist[lane % kSelCopies * kSelPitch + (image[u] >> 24)], 1);
+      } else {
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u)
+          if (u < used && competes(at(c0, used, u)) && (image[u] >> top) == prefix)
+            atomicAdd(&hist[(image[u] >> shift) & 4095u], 1);
+      }
     }
     __syncthreads();
-    // thread t holds bins 2047 - 2t, 2046 - 2t: keys above a bin by a prefix sum over the threads
-    const int b0 = 2047 - 2 * tid, n0 = hist[b0], n1 = hist[b0 - 1];
-    int sum = n0 + n1;
+    // a thread holds 4 bins (pass 0: the first 256 threads one), the highest first: keys above a bin by
+    // a prefix sum over the threads
+    const int b0 = pass == 0 ? 255 - tid : 4095 - 4 * tid;
+    int own[4] = {0, 0, 0, 0};
+    if (pass > 0) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) own[k] = hist[b0 - k];
+    } else if (tid < 256) {
+#pragma unroll
+      for (int v = 0; v < kSelCopies; ++v) own[0] += hist[v * kSelPitch + b0];
+    }
+    const int mine = own[0] + own[1] + own[2] + own[3];
+    int sum = mine;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-      const int x = __shfl_up(sum, off);
-      if (lane >= off) sum += x;
+      const int y = __shfl_up(sum, off);
+      if (lane >= off) sum += y;
     }
-    if (lane == 63) wave_sum[wave] = sum;
+    if (lane == 63) wave_sum[0][wave] = sum;
     __syncthreads();
-    int above = sum - n0 - n1;
-    for (int i = 0; i < wave; ++i) above += wave_sum[i];
-    if (above < need && above + n0 >= need) { s_digit = b0; s_need = need - above; }
-    else if (above + n0 < need && above + n0 + n1 >= need) { s_digit = b0 - 1; s_need = need - above - n0; }
+    int above = sum - mine;
+#pragma unroll
+    for (int i = 0; i < kSelWaves; ++i) above += i < wave ? wave_sum[0][i] : 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (above < need && above + own[k] >= need) { s_digit = b0 - k; s_need = need - above; }
+      above += own[k];
+    }
     __syncthreads();
     prefix = (prefix << bits) | (unsigned)s_digit;
     need = s_need;
     __syncthreads();
   }
   // kept of [lo, hi): images above `prefix`, and the first `need` equal to it (none at all when no
-  // key of the middle stays)
+  // key of the middle stays): every wave counts its own, the counts meet in LDS, and the keys go to
+  // their places.
   const bool some = p.budget > p.sink + p.recent;
-  const int per_wave = ((n + kSelWaves - 1) / kSelWaves + 63) & ~63;
-  const int w0 = wave * per_wave, w1 = min(n, w0 + per_wave);
-  int above = 0, equal = 0;
-  for (int i0 = w0; i0 < w1; i0 += 64) {
-    const int i = i0 + lane;
-    const bool in = i < w1, mid = in && i >= lo && i < hi;
-    const unsigned u = mid ? ordered(w[i]) : 0u;
-    above += wave_count(in && (!mid || (some && u > prefix)));
-    equal += wave_count(mid && some && u == prefix);
+  int above0 = 0, equal0 = 0, dropped_first = n;   // kept above / equal before this chunk
+  for (int c0 = 0, turn = 0; c0 < n; c0 += CHUNK, turn ^= 1) {
+    const int used = fetch(c0);
+    unsigned gt = 0, eq = 0;                       // bit u: this lane's key u
+    int above = 0, equal = 0;
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u)
+      if (u < used) {
+        const int i = at(c0, used, u);
+        const bool mid = competes(i);
+        const bool g = i < n && (!mid || (some && image[u] > prefix)), e = mid && some && image[u] == prefix;
+        gt |= (unsigned)g << u;
+        eq |= (unsigned)e << u;
+        above += wave_count(g);
+        equal += wave_count(e);
+      }
+    if (lane == 0) { wave_sum[turn][wave] = above; wave_sum2[turn][wave] = equal; }
+    __syncthreads();                               // (the two turns' counts alternate: one barrier a chunk)
+    int ga = above0, ea = equal0;
+#pragma unroll
+    for (int v = 0; v < kSelWaves; ++v) {
+      const int a = wave_sum[turn][v], e = wave_sum2[turn][v];
+      ga += v < wave ? a : 0;
+      ea += v < wave ? e : 0;
+      above0 += a;
+      equal0 += e;
+    }
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u)
+      if (u < used) {
+        const int i = at(c0, used, u);
+        const bool g = (gt >> u) & 1, e = (eq >> u) & 1;
+        const int erank = ea + lanes_below(e, lane);
+        const int place = ga + lanes_below(g, lane) + min(erank, need);
+        const bool keep = g || (e && erank < need);
+        if (keep) { kept[place] = i; wo[place] = x[u]; }
+        if (i < n && !keep) dropped_first = min(dropped_first, i);
+        ga += wave_count(g);
+        ea += wave_count(e);
+      }
   }
-  if (lane == 0) { wave_sum[wave] = above; wave_sum2[wave] = equal; }
-  __syncthreads();
-  int above0 = 0, equal0 = 0;
-  for (int i = 0; i < wave; ++i) { above0 += wave_sum[i]; equal0 += wave_sum2[i]; }
-  for (int i0 = w0; i0 < w1; i0 += 64) {
-    const int i = i0 + lane;
-    const bool in = i < w1, mid = in && i >= lo && i < hi;
-    const float x = in ? w[i] : 0.f;
-    const unsigned u = mid ? ordered(x) : 0u;
-    const bool eq = mid && some && u == prefix;
-    const bool gt = in && (!mid || (some && u > prefix));
-    const int erank = equal0 + lanes_below(eq, lane);
-    const bool keep = gt || (eq && erank < need);
-    const int place = above0 + lanes_below(gt, lane) + min(erank, need);
-    if (keep) { kept[place] = i; wo[place] = x; }
-    const uint64_t dropped = __ballot(in && !keep);
-    if (lane == 0 && dropped != 0) atomicMin(&s_first, i0 + __builtin_ctzll(dropped));
-    above0 += wave_count(gt);
-    equal0 += wave_count(eq);
-  }
-  for (int i = p.budget + tid; i < c.slots; i += kSelThreads) wo[i] = 0.f;
-  __syncthreads();
+  if (dropped_first < n) atomicMin(&s_first, dropped_first);
+  lds_barrier();                                   // (leaves the stores in flight)
   if (tid == 0) p.first[bh] = min(s_first, p.budget);   // keys below the first dropped one stay put
+  for (int i = p.budget + tid; i < c.slots; i += kSelThreads) wo[i] = 0.f;
 }
 
 // Moves rows list(i) -> base + i for i in [first, count) of one column slice; list(i) is a key >= base + i,
@@ -144,14 +205,21 @@ __device__ inline void move_rows(const KvCache& c, char* base_ptr, int bidb, int
   const bool col_ok = col + 8 * ((int)threadIdx.x % LANES) < c.d;
   bool ok[2][U];
   u32x4_t x[2][U];
-  auto load = [&](int i0, int b) {
+  int from[U];                                     // the next chunk's keys, read a chunk before their rows
+  auto look_up = [&](int i0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = i0 + u * ROWS + rl;
+      from[u] = i < count ? list(i) : -1;
+    }
+  };
+  auto load = [&](int b) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
       bool bad = false;
-      ok[b][u] = i < count && col_ok;
+      ok[b][u] = from[u] >= 0 && col_ok;
       if (!ok[b][u]) continue;
-      const int64_t off = slot_offset(c, bidb, list(i), bad);
+      const int64_t off = slot_offset(c, bidb, from[u], bad);
       ok[b][u] = !bad;
       if (!bad) x[b][u] = *(const u32x4_t*)(base_ptr + off * 2 + cb);
     }
@@ -171,13 +239,17 @@ __device__ inline void move_rows(const KvCache& c, char* base_ptr, int bidb, int
   };
 #pragma unroll
   for (int u = 0; u < U; ++u) x[0][u] = x[1][u] = u32x4_t{0u, 0u, 0u, 0u};
-  load(first, 0);
+  look_up(first);
+  load(0);
+  look_up(first + CHUNK);
   for (int i0 = first; i0 < count; i0 += 2 * CHUNK) {
-    load(i0 + CHUNK, 1);
+    load(1);
+    look_up(i0 + 2 * CHUNK);
     landed(0);
     lds_barrier();
     store(i0, 0);
-    load(i0 + 2 * CHUNK, 0);
+    load(0);
+    look_up(i0 + 3 * CHUNK);
     landed(1);
     lds_barrier();
     store(i0 + CHUNK, 1);
@@ -243,7 +315,11 @@ __global__ void __launch_bounds__(kMoveThreads) kv_commit_kernel(const KvCommitP
 
 void launch_kv_evict(const KvEvictParams& p, hipStream_t stream) {
   const KvCache& c = p.c;
-  hipLaunchKernelGGL(kv_select_kernel, dim3((unsigned)c.hk, (unsigned)c.b), dim3(kSelThreads), 0, stream, p);
+  // 32 keys a thread unroll to code that a small cache does not earn back (4k slots, 8 heads: 8 keys a
+  // thread 15.7 us, 32 keys 22.4; at 32k slots, 64 heads: 4 keys 47.8, 32 keys 38 us)
+  const dim3 heads((unsigned)c.hk, (unsigned)c.b);
+  if (c.slots <= 8 * kSelThreads) hipLaunchKernelGGL((kv_select_kernel<8>), heads, dim3(kSelThreads), 0, stream, p);
+  else hipLaunchKernelGGL((kv_select_kernel<32>), heads, dim3(kSelThreads), 0, stream, p);
   const int slices = (c.d + 8 * kEvictLanes - 1) / (8 * kEvictLanes);
   const int64_t grid = ((int64_t)c.b * c.hk + 7) / 8 * 8 * 2 * slices;
   if (grid > 0x7fffffff) throw std::runtime_error("kvcache evict: too many workgroups for one launch");
