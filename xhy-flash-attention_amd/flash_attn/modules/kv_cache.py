@@ -1,0 +1,57 @@
+"""The key/value cache of one attention layer, as ``MHA.forward(..., kv_cache=cache)`` uses it.
+
+    cache = KVCache(batch, slots, nheads_k, headdim, device="cuda", dtype=torch.bfloat16, track_weight=True)
+    y = mha(x, kv_cache=cache)                        # x: the prompt, or the next tokens
+    cache.accept(x.shape[1])
+    y = mha(drafts, kv_cache=cache, tree_mask=mask, depth=mask.sum(-1, dtype=torch.int32) - 1)
+    cache.commit(accepted)                            # of a tree of drafted tokens
+    cache.evict(budget, sink=4, recent=256)
+
+Lengths and positions live on the GPU; nothing here synchronises.
+"""
+import torch
+
+from flash_attn.kvcache_interface import flash_attn_kvcache_commit_, flash_attn_kvcache_evict_
+
+__all__ = ["KVCache"]
+
+
+class KVCache:
+    """k, v: (batch, slots, nheads_k, headdim), or pages with ``block_table`` (flash_attn_kvcache_func).
+
+    seqlens: int32 (batch,), the keys held; positions: int32 (batch,), the position of the next token, which
+    eviction leaves alone; most: no position is above it (known on the host: it sizes the rotary table,
+    which a capture into a graph should find large enough); attn_weight: fp32 (batch, nheads_k, slots)
+    with track_weight, else None."""
+
+    def __init__(self, batch_size, slots, nheads_k, headdim, device=None, dtype=None, track_weight=False):
+        self.k = torch.zeros(batch_size, slots, nheads_k, headdim, device=device, dtype=dtype)
+        self.v = torch.zeros_like(self.k)
+        self.block_table = None
+        self.seqlens = torch.zeros(batch_size, device=device, dtype=torch.int32)
+        self.positions = torch.zeros_like(self.seqlens)
+        self.most = 0
+        self.attn_weight = None
+        if track_weight:
+            self.attn_weight = torch.zeros(batch_size, nheads_k, slots, device=device, dtype=torch.float32)
+
+    def accept(self, count):
+        """Keeps all ``count`` tokens of the last call."""
+        self.seqlens = self.seqlens + count
+        self.positions = self.positions + count
+        self.most += count
+
+    def commit(self, accepted):
+        """Keeps the accepted ones (bool (batch, seqlen_q)) of the last call's tokens, in their order."""
+        seqlens = flash_attn_kvcache_commit_(self.k, self.v, self.seqlens, accepted, self.block_table, self.attn_weight)
+        self.positions = self.positions + (seqlens - self.seqlens)
+        self.seqlens = seqlens
+        self.most += accepted.shape[1]
+
+    def evict(self, budget, sink=0, recent=0):
+        """Shrinks sequences of more than ``budget`` keys; returns the slots the kept keys came from."""
+        if self.attn_weight is None:
+            raise RuntimeError("KVCache: eviction needs track_weight=True")
+        self.seqlens, self.attn_weight, kept = flash_attn_kvcache_evict_(
+            self.k, self.v, self.seqlens, self.attn_weight, budget, sink, recent, self.block_table)
+        return kept
