@@ -163,6 +163,12 @@ bool varlen_items_fit(int b, int nlev) {
 
 uint32_t* build_varlen_items(StreamScratch& buf, const int* cu, int b, int nh, int gdiv, int rows, int nlev,
                              bool reverse, long long max_items, hipStream_t stream) {
+  // A captured list has once faulted the forward that reads it when the graph was replayed, and no
+  // cause is known: such a capture is refused (a fixed-length launch, which needs no list, is not).
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  check(hipStreamIsCapturing(stream, &capture), "hipStreamIsCapturing");
+  if (capture != hipStreamCaptureStatusNone)
+    throw std::runtime_error("a variable-length launch with a device-built work list cannot be captured into a graph");
   if (!buf.alloc((size_t)(2 * max_items + 2) * sizeof(uint32_t), stream))
     throw std::runtime_error("flash_attn_fwd (asm path): hipMallocAsync (varlen work list) failed");
   uint32_t* tab = static_cast<uint32_t*>(buf.p);
