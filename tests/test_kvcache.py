@@ -53,6 +53,10 @@ REFUSED = [
     (dict(softmax_scale=-1.0), "positive and finite"),
     (dict(softmax_scale=float("nan")), "positive and finite"),
     (dict(q=torch.zeros(2, 3, 4, 64, dtype=BF, requires_grad=True)), "no backward"),
+    (dict(k_cache=torch.zeros(1, 50, 2, 64, dtype=BF).expand(2, -1, -1, -1),
+          v_cache=torch.zeros(1, 50, 2, 64, dtype=BF).expand(2, -1, -1, -1)), "not be expanded"),
+    (dict(attn_weight=torch.zeros(2, 1, 50).expand(-1, 2, -1)), "not be expanded"),
+    (dict(attn_weight=torch.zeros(2, 2, 50, requires_grad=True)), "no backward"),
     (dict(), "on the GPU"),
 ]
 
@@ -62,6 +66,31 @@ def test_attention_refuses(over, message):
     from flash_attn import flash_attn_kvcache_func
     with pytest.raises(RuntimeError, match=message):
         flash_attn_kvcache_func(**_args(**over))
+
+
+def test_shared_memory_is_refused():
+    from flash_attn import flash_attn_kvcache_commit_, flash_attn_kvcache_evict_, flash_attn_kvcache_func
+    from flash_attn.layers.qk_norm import apply_qk_norm_rotary_func
+    a = _args()
+    a["v_cache"] = a["k_cache"]
+    with pytest.raises(RuntimeError, match="share memory"):
+        flash_attn_kvcache_func(**a)
+    with pytest.raises(RuntimeError, match="share memory"):
+        flash_attn_kvcache_commit_(a["k_cache"], a["k_cache"].view_as(a["k_cache"]), a["cache_seqlens"],
+                                   torch.ones(2, 3, dtype=torch.bool))
+    one = torch.zeros(1, 50, 2, 64, dtype=BF).expand(2, -1, -1, -1)
+    with pytest.raises(RuntimeError, match="not be expanded"):
+        flash_attn_kvcache_evict_(one, one[:1].clone().expand(2, -1, -1, -1), a["cache_seqlens"], torch.zeros(2, 2, 50), 10)
+    a["k"] = a["v"] = None                         # nothing is written: read all the same
+    with pytest.raises(RuntimeError, match="on the GPU"):
+        flash_attn_kvcache_func(**a)
+    with pytest.raises(RuntimeError, match="share memory"):
+        apply_qk_norm_rotary_func(a["q"], a["q"], inplace=True)
+    with pytest.raises(RuntimeError, match="not be expanded"):
+        apply_qk_norm_rotary_func(a["q"][:, :, :1].expand(-1, -1, 4, -1), a["q"], inplace=True)
+    kv = torch.zeros(2, 3, 2, 4, 64, dtype=BF)     # halves of one tensor do not overlap
+    with pytest.raises(RuntimeError, match="on the GPU"):
+        apply_qk_norm_rotary_func(kv[:, :, 0], kv[:, :, 1], inplace=True)
 
 
 def test_commit_and_evict_refuse():

@@ -435,3 +435,30 @@ def test_deterministic_and_split_independent_of_room():
     for o in outs[2:]:
         torch.testing.assert_close(o[0].float(), outs[0][0].float(), atol=2.0 ** -11, rtol=2.0 ** -9)
         torch.testing.assert_close(o[1], outs[0][1], atol=2.0 ** -18, rtol=2.0 ** -18)
+
+
+def test_misaligned_contiguous_rows():
+    """q, k and v may start at any element: contiguous tensors off a 16-byte boundary give what aligned ones give."""
+    from flash_attn import flash_attn_kvcache_func
+    torch.manual_seed(0)
+    q, k, v = (torch.randn(2, 3, h, 64, device=DEV, dtype=torch.float16) for h in (4, 2, 2))
+    lens = torch.tensor([5, 33], device=DEV, dtype=torch.int32)
+
+    def off(t):
+        x = torch.empty(t.numel() + 3, device=DEV, dtype=t.dtype)[3:].view(t.shape)
+        return x.copy_(t)
+
+    caches = [torch.randn(2, 40, 2, 64, device=DEV, dtype=torch.float16) for _ in range(2)]
+    outs = []
+    for f in (lambda t: t, off):
+        kc, vc = (c.clone() for c in caches)
+        outs.append((flash_attn_kvcache_func(f(q), kc, vc, lens, k=f(k), v=f(v)), kc, vc))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
+def test_more_sequences_than_lanes():
+    """The scan over the lengths goes past 64 sequences."""
+    lens = [(37 * i) % 301 for i in range(150)]
+    _run(150, 3, 4, 2, 64, lens, torch.bfloat16, 0)
+    _run(150, 1, 2, 1, 128, lens, torch.float16, 32)

@@ -155,3 +155,34 @@ def test_refusals():
         MHA(64, 2, qk_norm=True, rotary_emb_dim=32, rotary_emb_scale_base=512)
     with pytest.raises(RuntimeError, match="track_weight"):
         cache.evict(4)
+
+
+def test_captured_decoding_goes_on():
+    """A decoding step with its accept, captured once: each replay stands one token further on."""
+    from flash_attn.modules.kv_cache import KVCache
+    m = _mha(4, 2, 32, 32)
+    x = torch.randn(2, 16, 128, device=DEV, dtype=torch.float16)
+    with torch.no_grad():
+        whole = m(x)
+        cache = KVCache(2, 64, 2, 32, device=DEV, dtype=torch.float16)
+        cache.most = 64                            # no position beyond it in any replay
+        y = m(x[:, :10], kv_cache=cache)
+        cache.accept(10)
+        token = x[:, 10:11].clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):              # (warm-up: stores the token, without keeping it)
+            m(token, kv_cache=cache)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step = m(token, kv_cache=cache)
+            cache.accept(1)
+        parts = [y]
+        for i in range(10, 16):
+            token.copy_(x[:, i:i + 1])
+            graph.replay()
+            parts.append(step.clone())
+            torch.cuda.synchronize()
+    assert cache.seqlens.tolist() == [16] * 2 and cache.positions.tolist() == [16] * 2
+    assert (torch.cat(parts, 1).float() - whole.float()).abs().le(_bound(m, x, whole)).all()

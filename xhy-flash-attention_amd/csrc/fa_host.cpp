@@ -3,8 +3,9 @@
 //
 // A decoding step launches kernels of 5 to 15 us; the same checks and calls through Python and ctypes took
 // 15 to 30 us a call, and a forward with its backward 180 us, which the GPU spent waiting.  Here they take
-// 5 to 10 us (45 us).  The kernels stay behind the C ABI of libflash_attn_mi355x.so: bind() is handed the
+// 6 to 11 us (83 us, most of it the autograd engine's).  The kernels stay behind the C ABI of libflash_attn_mi355x.so: bind() is handed the
 // addresses of its entry points by flash_attn_2_cuda, which loads it, so that one library serves both.
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -77,7 +78,22 @@ bool aligned(const Tensor& t) {
 void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
-Tensor vec_ok(const Tensor& t) { return aligned(t) ? t : t.contiguous(); }
+Tensor vec_ok(const Tensor& t) { return aligned(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+// t is written: an expanded tensor, or two that share elements, would be by several rows at once
+void check_writable(const char* op, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* a : ts) {
+    if (a == nullptr) continue;
+    TORCH_CHECK(at::has_internal_overlap(*a) != at::MemOverlap::Yes, op, ": written tensors must not be expanded");
+    for (const Tensor* b : ts) {
+      if (b == a) break;
+      if (b == nullptr) continue;
+      const auto overlap = at::get_overlap_status(*a, *b);
+      TORCH_CHECK(a->unsafeGetTensorImpl() != b->unsafeGetTensorImpl() && overlap != at::MemOverlapStatus::Full &&
+                      overlap != at::MemOverlapStatus::Partial,
+                  op, ": written tensors must not share memory");
+    }
+  }
+}
 
 // the last of the checks: everything on one GPU (its architecture is checked behind the C ABI)
 void check_device(const char* op, std::initializer_list<const Tensor*> ts) {
@@ -172,7 +188,9 @@ std::pair<Tensor, Tensor> kvcache(const Tensor& q_in, const Tensor& k_cache, con
                   "kvcache: k and v must have shape (batch, seqlen_q, nheads_k, headdim)");
       TORCH_CHECK(t->stride(3) == 1, "kvcache: k and v must have a contiguous last dimension");
     }
-  check_no_grad({&q_in, opt(k_in), opt(v_in), &k_cache, &v_cache});
+  check_no_grad({&q_in, opt(k_in), opt(v_in), &k_cache, &v_cache, opt(weight)});
+  if (k_in) check_writable("kvcache", {&k_cache, &v_cache, opt(weight)});
+  else check_writable("kvcache", {opt(weight)});
   OptTensor mask;
   int64_t mask_strides[2] = {0, 0};
   if (mask_in) {
@@ -225,7 +243,8 @@ Tensor commit(const Tensor& k_cache, const Tensor& v_cache, const Tensor& lens, 
   if (weight) c.limit(*weight);
   TORCH_CHECK(0 < sq && sq <= 8192 && sq <= c.slots, "kvcache: between 1 and min(8192, slots) drafted tokens");
   const Tensor accepted = flag_bytes(accepted_in, "accepted");
-  check_no_grad({&k_cache, &v_cache});
+  check_no_grad({&k_cache, &v_cache, opt(weight)});
+  check_writable("kvcache", {&k_cache, &v_cache, opt(weight)});
   check_device("kvcache", {&k_cache, &v_cache, &lens, opt(table), &accepted, opt(weight)});
   const c10::DeviceGuard guard(k_cache.device());
   Tensor out = at::empty_like(lens);
@@ -252,6 +271,7 @@ std::tuple<Tensor, Tensor, Tensor> evict(const Tensor& k_cache, const Tensor& v_
   TORCH_CHECK(c.b <= 65535, "kvcache: batch size must be at most 65535");
   c.limit(weight);
   check_no_grad({&k_cache, &v_cache, &weight});
+  check_writable("kvcache", {&k_cache, &v_cache});
   check_device("kvcache", {&k_cache, &v_cache, &lens, opt(table), &weight});
   const c10::DeviceGuard guard(k_cache.device());
   Tensor out = at::empty_like(lens);
@@ -430,6 +450,7 @@ struct QkNormRotary : torch::autograd::Function<QkNormRotary> {
 std::pair<Tensor, Tensor> norm_rotary(const Tensor& q, const Tensor& k, const OptTensor& wq, const OptTensor& wk,
                                       const OptTensor& cos, const OptTensor& sin, const OptTensor& pos, bool interleaved,
                                       double eps, bool inplace) {
+  if (inplace) check_writable("qk_norm_rotary", {&q, &k});
   check_norm(q, k, wq, wk, cos, sin, pos, eps);
   if (inplace) {
     bool grad = false;

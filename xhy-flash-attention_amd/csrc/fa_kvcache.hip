@@ -729,7 +729,9 @@ static void run_attn(const KvAttnParams& p, hipStream_t stream) {
   const int chunks = p.scores != nullptr ? (p.c.slots + 1023) / 1024 : 0;
   const int64_t merges = !may_cut(p) ? 0 : bh * (many ? (p.rows + kFewPieces - 1) / kFewPieces : p.rows);
   const int64_t tail = merges + bh * chunks;
-  if (tail > 0x7fffffff) throw std::runtime_error("kvcache attention: too many workgroups for one launch");
+  const int weight_chunks = p.weight != nullptr && p.scores == nullptr ? (p.c.slots + 127) / 128 : 0;
+  if (tail > 0x7fffffff || weight_chunks > 65535)
+    throw std::runtime_error("kvcache attention: too many workgroups for one launch");
   const dim3 g((unsigned)((p.shares + 7) / 8 * 8 * p.c.hk * p.m_tiles)), t(256), gt((unsigned)tail);
   switch (rows_per_unit(p.rows)) {
     case 32: hipLaunchKernelGGL((kv_attn_kernel<BF16, D, 1>), g, t, 0, stream, p); break;
@@ -738,9 +740,8 @@ static void run_attn(const KvAttnParams& p, hipStream_t stream) {
   }
   if (tail > 0 && many) hipLaunchKernelGGL((kv_merge_kernel<BF16, D, kFewPieces>), gt, t, 0, stream, p, (int)merges, chunks);
   else if (tail > 0) hipLaunchKernelGGL((kv_merge_kernel<BF16, D, 1>), gt, t, 0, stream, p, (int)merges, chunks);
-  if (p.weight != nullptr && p.scores == nullptr)
-    hipLaunchKernelGGL((kv_weight_kernel<BF16, D>), dim3((unsigned)bh, (unsigned)((p.c.slots + 127) / 128)), t, 0, stream,
-                       p);
+  if (weight_chunks > 0)
+    hipLaunchKernelGGL((kv_weight_kernel<BF16, D>), dim3((unsigned)bh, (unsigned)weight_chunks), t, 0, stream, p);
 }
 
 template <bool BF16>

@@ -7,7 +7,7 @@
 
 The cache is (batch, slots, nheads_k, headdim) or, with a block table, pages of (num_pages, page_size,
 nheads_k, headdim).  Lengths and block table stay on the device: no call synchronises, every call can be
-captured in a graph, and no kernel touches memory outside the cache whatever they hold.  The checks and
+captured in a graph (a written tensor may not be expanded or shared with another), and no kernel touches memory outside the cache whatever they hold.  The checks and
 allocations are in C++ (csrc/fa_host.cpp: a decoding step is short); the kernels are behind
 ``flash_attn_kvcache``, ``flash_attn_kvcache_commit`` and ``flash_attn_kvcache_evict`` (include/flash_attn.h); no reference counterpart (the reference's 2.0.8 API has no cache).
 """

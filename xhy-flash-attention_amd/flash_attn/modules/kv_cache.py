@@ -7,7 +7,8 @@
     cache.commit(accepted)                            # of a tree of drafted tokens
     cache.evict(budget, sink=4, recent=256)
 
-Lengths and positions live on the GPU; nothing here synchronises.
+Lengths and positions live on the GPU and are updated in place: nothing here synchronises, and a step
+captured into a graph goes on where its last replay stopped.
 """
 import torch
 
@@ -20,9 +21,10 @@ class KVCache:
     """k, v: (batch, slots, nheads_k, headdim), or pages with ``block_table`` (flash_attn_kvcache_func).
 
     seqlens: int32 (batch,), the keys held; positions: int32 (batch,), the position of the next token, which
-    eviction leaves alone; most: no position is above it (known on the host: it sizes the rotary table,
-    which a capture into a graph should find large enough); attn_weight: fp32 (batch, nheads_k, slots)
-    with track_weight, else None."""
+    eviction leaves alone; most: no position is above it (known on the host: it sizes the rotary table.
+    Replays of a graph do not count it up: set it to the longest length that they reach before the
+    capture, as a position outside the table gives NaN); attn_weight: fp32 (batch, nheads_k, slots) with
+    track_weight, else None."""
 
     def __init__(self, batch_size, slots, nheads_k, headdim, device=None, dtype=None, track_weight=False):
         self.k = torch.zeros(batch_size, slots, nheads_k, headdim, device=device, dtype=dtype)
@@ -37,21 +39,23 @@ class KVCache:
 
     def accept(self, count):
         """Keeps all ``count`` tokens of the last call."""
-        self.seqlens = self.seqlens + count
-        self.positions = self.positions + count
+        self.seqlens += count
+        self.positions += count
         self.most += count
 
     def commit(self, accepted):
         """Keeps the accepted ones (bool (batch, seqlen_q)) of the last call's tokens, in their order."""
         seqlens = flash_attn_kvcache_commit_(self.k, self.v, self.seqlens, accepted, self.block_table, self.attn_weight)
-        self.positions = self.positions + (seqlens - self.seqlens)
-        self.seqlens = seqlens
+        self.positions += seqlens - self.seqlens
+        self.seqlens.copy_(seqlens)
         self.most += accepted.shape[1]
 
     def evict(self, budget, sink=0, recent=0):
         """Shrinks sequences of more than ``budget`` keys; returns the slots the kept keys came from."""
         if self.attn_weight is None:
             raise RuntimeError("KVCache: eviction needs track_weight=True")
-        self.seqlens, self.attn_weight, kept = flash_attn_kvcache_evict_(
-            self.k, self.v, self.seqlens, self.attn_weight, budget, sink, recent, self.block_table)
+        seqlens, weight, kept = flash_attn_kvcache_evict_(self.k, self.v, self.seqlens, self.attn_weight, budget, sink,
+                                                          recent, self.block_table)
+        self.seqlens.copy_(seqlens)
+        self.attn_weight.copy_(weight)
         return kept
