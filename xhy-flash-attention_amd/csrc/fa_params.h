@@ -153,7 +153,7 @@ struct RotaryParams {
 // with element strides and a contiguous last dim.  Forward: q, k -> q_out, k_out.  Backward: also the
 // output gradients q_grad, k_grad; q_out, k_out receive dq, dk; dwq, dwk (optional) the gains' gradients
 // through the fp32 partials dw_part, kQkNormMaxBlocks x d.
-constexpr int kQkNormMaxBlocks = 1024;
+constexpr int kQkNormMaxBlocks = 768;
 struct QkNormTensor {
   const void* ptr;
   int64_t batch, row, head;
