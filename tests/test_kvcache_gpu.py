@@ -462,3 +462,10 @@ def test_more_sequences_than_lanes():
     lens = [(37 * i) % 301 for i in range(150)]
     _run(150, 3, 4, 2, 64, lens, torch.bfloat16, 0)
     _run(150, 1, 2, 1, 128, lens, torch.float16, 32)
+
+
+@pytest.mark.parametrize("page", [0, 24])
+@pytest.mark.parametrize("d", [40, 128, 256])
+def test_evict_many_heads(d, page):
+    """As many heads as take the whole-line column slices of the move."""
+    test_evict(16, d, [(97 * i) % 700 for i in range(16)], 150, 3, 20, page)

@@ -10,13 +10,16 @@
 //     found so far.  Weights crowd in a few exponents, so the first histogram has a copy for every two
 //     lanes.  One more pass counts, per wave over consecutive keys, those above and those equal;
 //     their prefix sums give every kept key its place, so the result is a function of the weights alone;
-//   * move: place i receives key kept[i] >= i.  A workgroup owns all rows of a 64-byte column slice of K
+//   * move: place i receives key kept[i] >= i.  A workgroup owns all rows of a 64- or 128-byte column slice of K
 //     or V of one (sequence, kv head) and walks the places upwards in chunks: the chunk's rows are in
 //     registers in every thread (barrier) before any of its places is written, and places below
 //     a chunk are never read by a later one, so in place needs no second buffer: each kept row
 //     is read once and written once.  The next chunk's rows are on their way over the barrier.
 // Commit is the move kernel with the list of the accepted drafted tokens, built in LDS by the workgroup
 // itself, at places lens[b] ...
+// Measured: 8 heads of 4.2k keys to 2k: select 15.7 us, bound by its passes' barriers on one CU a head, move
+// 6.5; 64 heads of 9k to 32k keys to 8k (paged, d = 128, fp16): select 38 us, move 129 us (0.54 GB, 4.2 TB/s in
+// scattered 256-byte rows, a copy's 5.2 in whole pages); commit of 128 x 64 drafted 8.8 us, of one sequence 3.0.
 #include <stdexcept>
 #include <string>
 
@@ -26,7 +29,6 @@ namespace fa {
 
 static constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
 static constexpr int kSelCopies = 32, kSelPitch = 257;   // histograms of the first pass, by lane (see below)
-static constexpr int kMoveThreads = 512;
 
 // 32-bit image of a weight: unsigned order = numeric order, NaN above +inf, -0 = +0
 __device__ inline unsigned ordered(float x) {
@@ -194,12 +196,17 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const KvEvictPar
   for (int i = p.budget + tid; i < c.slots; i += kSelThreads) wo[i] = 0.f;
 }
 
+// Threads and rows a thread: eviction walks thousands of rows (64 heads of 8k: 1024 threads 129 us, 512 172; two
+// or six rows 134), commit the accepted ones of a few dozen (128 x 64 drafted: 256 threads with one row
+// 8.8 us, with four 9.5; 512 with two 11.6, 1024 16.8).
+static constexpr int kEvictThreads = 1024, kEvictRows = 4, kCommitThreads = 256, kCommitLanes = 16, kCommitRows = 1;
+
 // Moves rows list(i) -> base + i for i in [first, count) of one column slice; list(i) is a key >= base + i,
 // ascending.  LANES lanes of 16 bytes a row, U rows a thread in flight, two chunks deep.
-template <int LANES, int U, typename List>
+template <int THREADS, int LANES, int U, typename List>
 __device__ inline void move_rows(const KvCache& c, char* base_ptr, int bidb, int col, int base, int first, int count,
                                  List list) {
-  constexpr int ROWS = kMoveThreads / LANES, CHUNK = ROWS * U;
+  constexpr int ROWS = THREADS / LANES, CHUNK = ROWS * U;
   const int rl = threadIdx.x / LANES;
   const int64_t cb = (int64_t)(col + 8 * (threadIdx.x % LANES)) * 2;
   const bool col_ok = col + 8 * ((int)threadIdx.x % LANES) < c.d;
@@ -256,10 +263,10 @@ __device__ inline void move_rows(const KvCache& c, char* base_ptr, int bidb, int
   }
 }
 
-// 64-byte column slices; the slices of a (sequence, kv head) sit 8 workgroups apart: the same XCD, so the
-// 128-byte lines that two of them share are fetched once
-static constexpr int kEvictLanes = 4;
-__global__ void __launch_bounds__(kMoveThreads) kv_evict_move_kernel(const KvEvictParams p, int slices) {
+// Column slices of LANES 16-byte pieces; the slices of a (sequence, kv head) sit 8 workgroups apart: the same
+// XCD, so lines that two of them share are fetched once
+template <int LANES>
+__global__ void __launch_bounds__(kEvictThreads) kv_evict_move_kernel(const KvEvictParams p, int slices) {
   const KvCache& c = p.c;
   const int per = 8 * 2 * slices;
   const int oct = blockIdx.x / per, rem = blockIdx.x - oct * per;
@@ -272,12 +279,11 @@ __global__ void __launch_bounds__(kMoveThreads) kv_evict_move_kernel(const KvEvi
   if (first >= count) return;
   char* base = (char*)(part >= slices ? c.v : c.k) + (int64_t)kvh * c.head * 2;
   const int* kept = p.kept + (int64_t)bh * p.budget;
-  move_rows<kEvictLanes, 4>(c, base, bidb, part % slices * kEvictLanes * 8, 0, first, count,
+  move_rows<kEvictThreads, LANES, kEvictRows>(c, base, bidb, part % slices * LANES * 8, 0, first, count,
                             [&](int i) { return kept[i]; });
 }
 
-static constexpr int kCommitLanes = 16;
-__global__ void __launch_bounds__(kMoveThreads) kv_commit_kernel(const KvCommitParams p, int slices) {
+__global__ void __launch_bounds__(kCommitThreads) kv_commit_kernel(const KvCommitParams p, int slices) {
   const KvCache& c = p.c;
   extern __shared__ int list[];                   // the accepted tokens, ascending
   __shared__ int s_count;
@@ -300,11 +306,11 @@ __global__ void __launch_bounds__(kMoveThreads) kv_commit_kernel(const KvCommitP
   if (part == 0 && kvh == 0 && threadIdx.x == 0) p.lens_out[bidb] = ok ? len + count : len;
   if (!ok) return;
   char* base = (char*)(part >= slices ? c.v : c.k) + (int64_t)kvh * c.head * 2;
-  move_rows<kCommitLanes, 2>(c, base, bidb, part % slices * kCommitLanes * 8, len, 0, count,
+  move_rows<kCommitThreads, kCommitLanes, kCommitRows>(c, base, bidb, part % slices * kCommitLanes * 8, len, 0, count,
                              [&](int i) { return len + list[i]; });
   if (p.weight != nullptr && part == 0) {
     float* w = p.weight + (int64_t)bidb * p.w_batch + (int64_t)kvh * p.w_head + len;
-    for (int i0 = 0; i0 < p.sq; i0 += kMoveThreads) {
+    for (int i0 = 0; i0 < p.sq; i0 += kCommitThreads) {
       const int i = i0 + (int)threadIdx.x;
       const float x = i < count ? w[list[i]] : 0.f;
       __syncthreads();                            // (waits for the loads: sources lie at or above i)
@@ -320,10 +326,15 @@ void launch_kv_evict(const KvEvictParams& p, hipStream_t stream) {
   const dim3 heads((unsigned)c.hk, (unsigned)c.b);
   if (c.slots <= 8 * kSelThreads) hipLaunchKernelGGL((kv_select_kernel<8>), heads, dim3(kSelThreads), 0, stream, p);
   else hipLaunchKernelGGL((kv_select_kernel<32>), heads, dim3(kSelThreads), 0, stream, p);
-  const int slices = (c.d + 8 * kEvictLanes - 1) / (8 * kEvictLanes);
-  const int64_t grid = ((int64_t)c.b * c.hk + 7) / 8 * 8 * 2 * slices;
+  // 128-byte slices (whole lines), or 64-byte ones where those leave CUs without a workgroup (64 heads of 8k
+  // kept keys: 128 bytes 129 us, 64 bytes 160; 8 heads of 2k: 8.9, 6.5 us)
+  const int64_t heads8 = ((int64_t)c.b * c.hk + 7) / 8 * 8;
+  const bool wide = heads8 * 2 * ((c.d + 63) / 64) >= 256;
+  const int slices = wide ? (c.d + 63) / 64 : (c.d + 31) / 32;
+  const int64_t grid = heads8 * 2 * slices;
   if (grid > 0x7fffffff) throw std::runtime_error("kvcache evict: too many workgroups for one launch");
-  hipLaunchKernelGGL(kv_evict_move_kernel, dim3((unsigned)grid), dim3(kMoveThreads), 0, stream, p, slices);
+  if (wide) hipLaunchKernelGGL((kv_evict_move_kernel<8>), dim3((unsigned)grid), dim3(kEvictThreads), 0, stream, p, slices);
+  else hipLaunchKernelGGL((kv_evict_move_kernel<4>), dim3((unsigned)grid), dim3(kEvictThreads), 0, stream, p, slices);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) throw std::runtime_error(std::string("kvcache evict launch: ") + hipGetErrorString(e));
 }
@@ -333,7 +344,7 @@ void launch_kv_commit(const KvCommitParams& p, hipStream_t stream) {
   const int slices = (c.d + 8 * kCommitLanes - 1) / (8 * kCommitLanes);
   const int64_t grid = (int64_t)c.b * c.hk * 2 * slices;
   if (grid > 0x7fffffff) throw std::runtime_error("kvcache commit: too many workgroups for one launch");
-  hipLaunchKernelGGL(kv_commit_kernel, dim3((unsigned)grid), dim3(kMoveThreads), (unsigned)p.sq * sizeof(int), stream,
+  hipLaunchKernelGGL(kv_commit_kernel, dim3((unsigned)grid), dim3(kCommitThreads), (unsigned)p.sq * sizeof(int), stream,
                      p, slices);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) throw std::runtime_error(std::string("kvcache commit launch: ") + hipGetErrorString(e));
