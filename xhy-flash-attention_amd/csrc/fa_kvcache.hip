@@ -532,42 +532,57 @@ __global__ void __launch_bounds__(256) kv_merge_kernel(const KvAttnParams p, int
     if (j0 >= total) return;
     const Pieces pc(p, sh, lane, bidb, len);       // (stored scores: one tile of rows, unit = kv head)
     __shared__ float s_lse[kScoreRows];
-    for (int r = threadIdx.x >> 6; r < p.rows; r += 4) {
-      float x;
-      if (pc.first < pc.last) {
-        float m = kNegInf, l = 0.f;
-        for (int s = pc.first + lane; s <= pc.last; s += 64) m = fmaxf(m, p.part_lse[pc.row(p, s, kvh, r)]);
+    // the first rows' scores and the weights are on their way over the LSE
+    constexpr int kAhead = 4;
+    const bool has = j < total;
+    const float* sc = p.scores + (int64_t)bh * p.rows * p.score_pitch + (has ? j : 0);
+    float* w = p.weight + (int64_t)bidb * p.w_batch + (int64_t)kvh * p.w_head + (has ? j : 0);
+    f32x4_t ahead[kAhead], sum;
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
-        for (int s = pc.first + lane; s <= pc.last; s += 64) {
+    for (int i = 0; i < kAhead; ++i) ahead[i] = *(const f32x4_t*)(sc + (int64_t)min(i, p.rows - 1) * p.score_pitch);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] = j + e < total ? w[e] : 0.f;
+    // eight threads a row, all rows at once
+    const int r = threadIdx.x >> 3, g = threadIdx.x & 7;
+    static_assert(kScoreRows <= 256 / 8, "a row has eight threads");
+    float m = kNegInf, l = 0.f;
+    auto join = [&](float m2, float l2) {          // (equal maxima, both -inf among them: no difference taken; NaN stays)
+      const float top = fmaxf(m, m2);
+      l = l * (m == top ? 1.f : fast_exp2(m - top)) + l2 * (m2 == top ? 1.f : fast_exp2(m2 - top));
+      m = top;
+    };
+    if (pc.first < pc.last) {
+      if (r < p.rows)
+        for (int s = pc.first + g; s <= pc.last; s += 8) {
           const float y = p.part_lse[pc.row(p, s, kvh, r)];
-          l += y == kNegInf ? 0.f : fast_exp2(y - m);
+          if (y != kNegInf) join(y, 1.f);
         }
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off);
-        x = l == 0.f ? kNegInf : m + __log2f(l);
-      } else {
-        const int t = r / p.group, head = kvh * p.group + r - t * p.group;
-        x = p.lse[((int64_t)bidb * p.h + head) * p.sq + t] * kLog2e;
-        if (x == -kNegInf) x = kNegInf;
+      for (int off = 4; off > 0; off >>= 1) {
+        const float m2 = __shfl_xor(m, off), l2 = __shfl_xor(l, off);
+        join(m2, l2);
       }
-      if (lane == 0) s_lse[r] = x;
+      if (g == 0 && r < p.rows) s_lse[r] = l == 0.f ? kNegInf : m + __log2f(l);
+    } else if (g == 0 && r < p.rows) {
+      const int t = r / p.group, head = kvh * p.group + r - t * p.group;
+      const float x = p.lse[((int64_t)bidb * p.h + head) * p.sq + t] * kLog2e;
+      s_lse[r] = x == -kNegInf ? kNegInf : x;
     }
     __syncthreads();
-    if (j >= total) return;
-    const float* sc = p.scores + (int64_t)bh * p.rows * p.score_pitch + j;
-    f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int r = 0; r < p.rows; ++r) {
-      const f32x4_t x = *(const f32x4_t*)(sc + (int64_t)r * p.score_pitch);
-      const float le = s_lse[r];
+    if (!has) return;
+    f32x4_t add = {0.f, 0.f, 0.f, 0.f};
+    auto row_adds = [&](const f32x4_t& x, float le) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += x[e] == kNegInf ? 0.f : fast_exp2(x[e] - le);
-    }
-    float* w = p.weight + (int64_t)bidb * p.w_batch + (int64_t)kvh * p.w_head + j;
+      for (int e = 0; e < 4; ++e) add[e] += x[e] == kNegInf ? 0.f : fast_exp2(x[e] - le);
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (i < p.rows) row_adds(ahead[i], s_lse[i]);
+#pragma unroll 4
+    for (int i = kAhead; i < p.rows; ++i) row_adds(*(const f32x4_t*)(sc + (int64_t)i * p.score_pitch), s_lse[i]);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (j + e < total) w[e] += sum[e];
+      if (j + e < total) w[e] = sum[e] + add[e];
     return;
   }
 
