@@ -225,10 +225,18 @@ __global__ void __launch_bounds__(256, groups_per_cu(D, WM)) kv_attn_kernel(cons
         }
       } else {
         const int ln = opaque(lane), ck = chunk_ok ? chunk : 0;
+        int64_t at_row[St::NI];                    // (all looked up before the first load)
+        if (p.even) {
+#pragma unroll
+          for (int i = 0; i < St::NI; ++i) at_row[i] = where + (j0 + St::row(i, ln) < len ? St::row(i, ln) * c.row : 0);
+        } else {
+#pragma unroll
+          for (int i = 0; i < St::NI; ++i) at_row[i] = shfl64(where, St::row(i, ln));
+        }
 #pragma unroll
         for (int i = 0; i < St::NI; ++i) {
-          const int jr = St::row(i, ln), u = j0 + jr - len;
-          const int64_t off = (p.even ? where + (u < 0 ? jr * c.row : 0) : shfl64(where, jr)) + ck;
+          const int u = j0 + St::row(i, ln) - len;
+          const int64_t off = at_row[i] + ck;
           const int64_t fresh = has_new && u >= 0 ? -1 : 0;   // (selected by bits: no branches)
           const int64_t uc = min(max(u, 0), p.sq - 1);
           const int64_t ka = (int64_t)(kc + off), kb = (int64_t)(kn + uc * p.kn_row + ck);
