@@ -179,8 +179,9 @@ __global__ void __launch_bounds__(256, groups_per_cu(D, WM)) kv_attn_kernel(cons
     const int old = has_new ? min(len, total) : total;   // keys that come from the cache
     const int bh = bidb * c.hk + kvh;
 
-    const int row = (mt * WM + wm) * 32 + r;       // this lane's row
-    const bool row_ok = row < p.rows;
+    const int rows_here = min(p.tile_rows, p.rows - mt * p.tile_rows);
+    const int row = mt * p.tile_rows + wm * 32 + r;   // this lane's row
+    const bool row_ok = wm * 32 + r < rows_here;
     const int tok = row_ok ? row / p.group : 0, gh = row_ok ? row - tok * p.group : 0;
 
     i16x8_t qf[KS];
@@ -303,7 +304,7 @@ __global__ void __launch_bounds__(256, groups_per_cu(D, WM)) kv_attn_kernel(cons
     };
     // one 32-key subtile in LDS: wave `sub`'s, first key j0
     auto compute = [&](int sub, int j0) {
-      if (WM > 1 && j0 >= total) return;           // (WM = 1: every step stores, see below)
+      if (WM > 1 && (j0 >= total || wm * 32 >= rows_here)) return;   // (WM = 1: every step stores, see below)
       const int tile = sub * 2 * TILE;
       const TileAddr ta(lb, tile);
       f32x16_t s;
@@ -436,7 +437,6 @@ __global__ void __launch_bounds__(256, groups_per_cu(D, WM)) kv_attn_kernel(cons
 
     const bool whole = s0 == 0 && s1 == steps;     // else a partial: slot 1 where the unit begins, 0 behind
     const int64_t slot = ((int64_t)share * units + unit) * 2 + (s0 == 0 ? 1 : 0);
-    const int rows_here = min(32 * WM, p.rows - mt * WM * 32);
     for (int i = tid; i < rows_here * CH; i += 256) {
       const int rl = i / CH, ch = i - rl * CH;
       const int w0 = rl >> 5, rr = rl & 31;        // waves w0, w0 + WM, ... hold the row
@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(256, groups_per_cu(D, WM)) kv_attn_kernel(cons
       const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[e] *= inv;
-      const int rg = mt * WM * 32 + rl, t = rg / p.group;
+      const int rg = mt * p.tile_rows + rl, t = rg / p.group;
       if (sm_odd[0] | sm_odd[1] | sm_odd[2] | sm_odd[3]) {
         for (int j = max(len, s0 * kStep); j < min(total, s1 * kStep); ++j) {
           bool out = false;
@@ -710,12 +710,15 @@ __global__ void __launch_bounds__(256) kv_weight_kernel(const KvAttnParams p) {
 // Rows of a unit, and the shares: as many as make the units the resident workgroups of the chip, four
 // rounds of them when a share alone has more than a quarter; fewer when there are not as many steps.
 // (Two or four rounds of smaller shares balance better but pay each a start and a merge: 5 to 10 % slower.)
+// Rows of several tiles are dealt evenly, in wholes of a wave's 32; the waves left over stage their keys only
+// (48 tokens x 4 heads, 16 x 4k keys: 96 + 96 rows 163 us, 128 + 64 171, and 183 with those waves computing
+// too; three tiles of 64 250).
 static int rows_per_unit(int rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
 void kv_attn_plan(KvAttnParams& p) {
   const int per = rows_per_unit(p.rows);
   p.m_tiles = (p.rows + per - 1) / per;
-  p.tile_rows = std::min(per, p.rows);
+  p.tile_rows = std::min(p.rows, ((p.rows + p.m_tiles - 1) / p.m_tiles + 31) / 32 * 32);
   const int64_t units = (int64_t)p.c.hk * p.m_tiles, steps = (int64_t)p.c.b * ((p.c.slots + kStep - 1) / kStep);
   if (steps > 0x7fffffff || units > 0xffffff) throw std::runtime_error("kvcache attention: too many keys for one launch");
   const int dd = p.c.d <= 64 ? 64 : p.c.d <= 128 ? 128 : 256;
