@@ -273,3 +273,27 @@ def test_module_and_refusals():
         _func()(q, k, m.q_weight, m.k_weight, inplace=True)
     with pytest.raises(RuntimeError, match="fewer rows"):
         _func()(q, k, None, None, cos[:8], sin[:8])
+
+
+def test_capture_beside_an_eager_graph_is_refused():
+    """The accumulators that an eager graph of the same leaves keeps alive belong to its stream, which a captured
+    backward could not leave: the captured forward is refused, and taken once that graph is gone."""
+    q, k = (t.contiguous() for t in _make(1, 9, 4, 2, 64, torch.bfloat16))
+    cos, sin = _table(9, 64, torch.float32)
+    w = torch.ones(64, device=DEV, requires_grad=True)
+    eager = _func()(q, k, w, w, cos, sin)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        with pytest.raises(RuntimeError, match="eager graph of the same leaves"):
+            _func()(q, k, w, w, cos, sin)
+        with torch.no_grad():                      # nothing to differentiate: nothing to refuse
+            _func()(q, k, w, w, cos, sin)
+    want = [t.detach().clone() for t in eager]
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _func()(q, k, w, w, cos, sin)
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))

@@ -447,6 +447,21 @@ struct QkNormRotary : torch::autograd::Function<QkNormRotary> {
   }
 };
 
+// A gradient accumulator that an eager graph keeps alive belongs to that graph's stream.  A backward that is
+// being captured would make this stream part of the capture, which torch cannot end: the process does.
+void check_capture(std::initializer_list<const Tensor*> ts) {
+  const auto stream = c10::hip::getCurrentHIPStream((*ts.begin())->device().index());
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+  for (const Tensor* t : ts) {
+    if (t == nullptr || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto of = node ? node->stream() : std::nullopt;
+    TORCH_CHECK(!of || of->id() == stream.id(),
+                "qk_norm_rotary: captured while an eager graph of the same leaves is alive; let go of its outputs first");
+  }
+}
+
 std::pair<Tensor, Tensor> norm_rotary(const Tensor& q, const Tensor& k, const OptTensor& wq, const OptTensor& wk,
                                       const OptTensor& cos, const OptTensor& sin, const OptTensor& pos, bool interleaved,
                                       double eps, bool inplace) {
@@ -462,6 +477,7 @@ std::pair<Tensor, Tensor> norm_rotary(const Tensor& q, const Tensor& k, const Op
     written(k);
     return {q, k};
   }
+  if (at::GradMode::is_enabled()) check_capture({&q, &k, opt(wq), opt(wk)});
   auto out = QkNormRotary::apply(q, k, wq, wk, cos, sin, pos, interleaved, eps);
   return {out[0], out[1]};
 }

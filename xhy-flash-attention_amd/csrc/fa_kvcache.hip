@@ -32,6 +32,11 @@
 // added to the rows that do (a rare path, looked for in steps with drafted keys only).
 // Keys past a sequence's end load as zeros, so no slot behind it reaches a result.  A sequence whose
 // length does not leave room for the drafted tokens, or that names a page outside the cache, gives NaN.
+//
+// Measured, 32 / 8 heads of 128: 8 sequences of 20k to 32k keys with weights 204 + 14 us (4.4 TB/s of K and V; a
+// step's hand-over through LDS and its products keep a workgroup from more); 4k keys of one sequence 12 + 4 us
+// (latency); 48 drafted tokens over 16 sequences of up to 8k keys in pages of 64: 164 + 12 us under the profiler,
+// 150 in all without it (softmax and products of 96-row tiles, two waves a SIMD).
 #include <algorithm>
 #include <stdexcept>
 #include <string>
@@ -711,7 +716,7 @@ __global__ void __launch_bounds__(256) kv_weight_kernel(const KvAttnParams p) {
 // rounds of them when a share alone has more than a quarter; fewer when there are not as many steps.
 // (Two or four rounds of smaller shares balance better but pay each a start and a merge: 5 to 10 % slower.)
 // Rows of several tiles are dealt evenly, in wholes of a wave's 32; the waves left over stage their keys only
-// (48 tokens x 4 heads, 16 x 4k keys: 96 + 96 rows 163 us, 128 + 64 171, and 183 with those waves computing
+// (48 tokens x 4 heads, 16 sequences of up to 8k keys: 96 + 96 rows 163 us, 128 + 64 171, and 183 with those waves computing
 // too; three tiles of 64 250).
 static int rows_per_unit(int rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 

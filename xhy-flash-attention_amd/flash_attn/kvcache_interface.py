@@ -7,13 +7,16 @@
 
 The cache is (batch, slots, nheads_k, headdim) or, with a block table, pages of (num_pages, page_size,
 nheads_k, headdim).  Lengths and block table stay on the device: no call synchronises, every call can be
-captured in a graph (a written tensor may not be expanded or shared with another), and no kernel touches memory outside the cache whatever they hold.  The checks and
-allocations are in C++ (csrc/fa_host.cpp: a decoding step is short); the kernels are behind
-``flash_attn_kvcache``, ``flash_attn_kvcache_commit`` and ``flash_attn_kvcache_evict`` (include/flash_attn.h); no reference counterpart (the reference's 2.0.8 API has no cache).
+captured in a graph, and no kernel touches memory outside the cache whatever they hold.  A tensor that a
+call writes may not be expanded or share memory with another that it writes.  The checks and allocations
+are in C++ (csrc/fa_host.cpp: a decoding step is short); the kernels are behind ``flash_attn_kvcache``,
+``flash_attn_kvcache_commit`` and ``flash_attn_kvcache_evict`` (include/flash_attn.h); no reference
+counterpart (the reference's 2.0.8 API has no cache).
 """
 import flash_attn_2_cuda as _ext
 
 __all__ = ["flash_attn_kvcache_func", "flash_attn_kvcache_commit_", "flash_attn_kvcache_evict_"]
+
 
 def flash_attn_kvcache_func(q, k_cache, v_cache, cache_seqlens, k=None, v=None, block_table=None, tree_mask=None,
                             softmax_scale=None, attn_weight=None, return_softmax_lse=False):

@@ -34,7 +34,9 @@ def apply_qk_norm_rotary_func(q: torch.Tensor, k: torch.Tensor, q_weight: Option
         interleaved: rotate adjacent columns (GPT-J) instead of the two halves (GPT-NeoX).
         inplace: write over q and k (inference: refused when a gradient is asked for).
     Returns q and k normalised and rotated, one rounding from fp32.  Differentiable (once) in q, k and
-    the weights; the weights' gradients are summed in a fixed order."""
+    the weights; the weights' gradients are summed in a fixed order.  Forward and backward can be captured in
+    a graph; a capture is refused while an eager graph of the same leaves is alive (its gradient accumulators
+    would draw their stream into the capture)."""
     return _ext.host_module().norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, interleaved, eps,
                                           inplace)
 
