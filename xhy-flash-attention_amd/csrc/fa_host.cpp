@@ -3,7 +3,7 @@
 //
 // A decoding step launches kernels of 5 to 15 us; the same checks and calls through Python and ctypes took
 // 15 to 30 us a call, and a forward with its backward 180 us, which the GPU spent waiting.  Here they take
-// 6 to 11 us (83 us, most of it the autograd engine's).  The kernels stay behind the C ABI of libflash_attn_mi355x.so: bind() is handed the
+// 5 to 11 us (50 to 85 us by machine, most of it the autograd engine's).  The kernels stay behind the C ABI of libflash_attn_mi355x.so: bind() is handed the
 // addresses of its entry points by flash_attn_2_cuda, which loads it, so that one library serves both.
 #include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
@@ -467,17 +467,23 @@ std::pair<Tensor, Tensor> norm_rotary(const Tensor& q, const Tensor& k, const Op
                                       double eps, bool inplace) {
   if (inplace) check_writable("qk_norm_rotary", {&q, &k});
   check_norm(q, k, wq, wk, cos, sin, pos, eps);
-  if (inplace) {
-    bool grad = false;
+  bool grad = false;
+  if (at::GradMode::is_enabled())
     for (const Tensor* t : {&q, &k, opt(wq), opt(wk)}) grad = grad || (t != nullptr && t->requires_grad());
-    TORCH_CHECK(!(grad && at::GradMode::is_enabled()),
-                "qk_norm_rotary: inplace=True is for inference; the backward needs the inputs");
+  if (inplace) {
+    TORCH_CHECK(!grad, "qk_norm_rotary: inplace=True is for inference; the backward needs the inputs");
     norm_forward(NormArgs(q, k, wq, wk, cos, sin, pos), q, k, interleaved, eps);
     written(q);
     written(k);
     return {q, k};
   }
-  if (at::GradMode::is_enabled()) check_capture({&q, &k, opt(wq), opt(wk)});
+  if (!grad) {   // (a decoding step waits for the host: none of autograd's part then)
+    const c10::DeviceGuard guard(q.device());
+    Tensor q_out = at::empty(q.sizes(), q.options()), k_out = at::empty(k.sizes(), k.options());
+    norm_forward(NormArgs(q, k, wq, wk, cos, sin, pos), q_out, k_out, interleaved, eps);
+    return {q_out, k_out};
+  }
+  check_capture({&q, &k, opt(wq), opt(wk)});
   auto out = QkNormRotary::apply(q, k, wq, wk, cos, sin, pos, interleaved, eps);
   return {out[0], out[1]};
 }
