@@ -3,8 +3,9 @@
 //
 // A decoding step launches kernels of 5 to 15 us; the same checks and calls through Python and ctypes took
 // 15 to 30 us a call, and a forward with its backward 180 us, which the GPU spent waiting.  Here they take
-// 5 to 11 us (50 to 85 us by machine, most of it the autograd engine's).  The kernels stay behind the C ABI of libflash_attn_mi355x.so: bind() is handed the
-// addresses of its entry points by flash_attn_2_cuda, which loads it, so that one library serves both.
+// 6 to 12 us (50 to 90 us by machine, of which a product of two tensors and its gradient takes half).  The
+// kernels stay behind the C ABI of libflash_attn_mi355x.so: bind() is handed the addresses of its entry points
+// by flash_attn_2_cuda, which loads it, so that one library serves both.
 #include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
