@@ -1,5 +1,5 @@
-// Addressing of the key/value cache (KvCache, fa_params.h), shared by the attention, eviction and commit
-// kernels.
+// Addressing of the key/value cache (KvCache, fa_params.h) and of the tree mask, shared by the attention, eviction
+// and commit kernels.
 #pragma once
 
 #include "fa_common.h"
@@ -18,6 +18,13 @@ __host__ __device__ inline int64_t slot_offset(const KvCache& c, int bidb, int j
   const bool in = pg >= 0 && pg < c.num_pages;
   if (!in) bad = true;
   return (int64_t)(in ? pg : 0) * c.batch + (int64_t)(j - blk * c.page) * c.row;
+}
+
+// The tree mask of a sequence is sq rows of sq bytes, mask_row apart: its bytes, and the byte that says whether
+// token t sees key j (outside the mask for a key that is no drafted one: cached, or behind the last)
+__host__ __device__ inline int mask_bytes(int sq, int mask_row) { return (sq - 1) * mask_row + sq; }
+__host__ __device__ inline int mask_offset(int t, int j, int len, int total, int mask_row, int outside) {
+  return j >= len && j < total ? t * mask_row + j - len : outside;
 }
 
 }  // namespace fa

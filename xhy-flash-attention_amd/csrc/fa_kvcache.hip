@@ -299,10 +299,12 @@ __global__ void __launch_bounds__(256, groups_per_cu(D, WM)) kv_attn_kernel(cons
         uniform_rsrc(p.scores != nullptr ? p.scores + (int64_t)bh * p.rows * p.score_pitch : p.lse,
                   p.scores != nullptr ? (int)(p.rows * p.score_pitch * 4) : 0);
 
-    // whether token t sees key j: its mask byte (branch-free), and what to make of it
-    const buf_rsrc_t rmask = uniform_rsrc(p.mask + (int64_t)bidb * p.mask_batch, p.mask != nullptr ? kFar : 0);
+    // whether token t sees key j: its mask byte (branch-free; keys that are not drafted are asked for too, and
+    // read nothing), and what to make of it
+    const buf_rsrc_t rmask = uniform_rsrc(p.mask + (int64_t)bidb * p.mask_batch,
+                                          p.mask != nullptr ? mask_bytes(p.sq, (int)p.mask_row) : 0);
     auto mask_byte = [&](int t, int j) {
-      return (unsigned)__builtin_amdgcn_raw_buffer_load_b8(rmask, j >= len ? t * (int)p.mask_row + j - len : kFar, 0, 0);
+      return (unsigned)__builtin_amdgcn_raw_buffer_load_b8(rmask, mask_offset(t, j, len, total, (int)p.mask_row, kFar), 0, 0);
     };
     auto sees = [&](int t, int j, unsigned byte) {
       return (j < total) & ((j < len) | (byte != 0) | ((p.mask == nullptr) & (j - len <= t)));
