@@ -268,12 +268,13 @@ __global__ void __launch_bounds__(256, groups_per_cu(D, WM)) kv_attn_kernel(cons
         for (int i = 0; i < St::NI; ++i) {
           const int off = panel_off(St::row(i, ln), St::chunk(ln), NR);
           const unsigned keep = chunk_ok && j0 + St::row(i, ln) < total ? ~0u : 0u;
+          const unsigned drafted = j0 + St::row(i, ln) >= len ? ~0u : 0u;
           u32x4_t kx, vx;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             kx[e] = st.k[i][e] & keep;
             vx[e] = st.v[i][e] & keep;
-            odd |= odd_pair<BF16>(vx[e]);
+            odd |= odd_pair<BF16>(vx[e]) & drafted;
           }
           *(u32x4_t*)(mine + off) = kx;
           *(u32x4_t*)(mine + TILE + off) = vx;
@@ -281,7 +282,8 @@ __global__ void __launch_bounds__(256, groups_per_cu(D, WM)) kv_attn_kernel(cons
         if (j0 + 32 > len && __any(odd != 0)) {    // (rare: through LDS, sparing the registers)
           found_odd = true;
 #pragma unroll 1
-          for (int i = lane; i < D / 32 * 256; i += 64) {   // 256 pairs of words a panel
+          for (int i = lane; i < D / 32 * 256; i += 64) {   // 256 pairs of words a panel, 8 a row
+            if (j0 + ((i & 255) >> 3) < len) continue;      // (cached: every row sees it)
             u32x2_t* const x = (u32x2_t*)(mine + TILE + (i >> 8) * NR * 64) + (i & 255);
             *x = u32x2_t{(*x)[0] & ~odd_pair<BF16>((*x)[0]), (*x)[1] & ~odd_pair<BF16>((*x)[1])};
           }
