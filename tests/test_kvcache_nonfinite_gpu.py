@@ -55,3 +55,25 @@ def test_cached_and_drafted_values_in_one_step(sq):
     want[0, :, :, 100] = torch.where(see, float("nan"), clean[0, :, :, 100].float())
     torch.testing.assert_close(out, want, rtol=0, atol=0, equal_nan=True)
     assert see.any() and not see.all()
+
+
+@pytest.mark.parametrize("sq", [4, 40])
+@pytest.mark.parametrize("new", [True, False])
+@pytest.mark.parametrize("n", [3, 1000])
+def test_a_weight_of_zero_makes_infinity_nan(n, new, sq):
+    """A drafted key that a row sees with a weight that is zero in fp32 (2^-1000 of the largest): 0 x inf."""
+    from flash_attn import flash_attn_kvcache_func
+    torch.manual_seed(0)
+    hk, d = 2, 64
+    lens = torch.tensor([n], device=DEV, dtype=torch.int32)
+    kc, vc, _ = _cache(1, n + sq, hk, d, torch.float16, 0)
+    q = torch.zeros(1, sq, hk, d, device=DEV, dtype=torch.float16)
+    k, v = (torch.randn(1, sq, hk, d, device=DEV).half() for _ in range(2))
+    q[..., 0], kc[..., 0], k[..., 0] = 8, 0, 0
+    k[0, 1, 0, 0] = -700                   # head 0: score -8 x 700 / 8 = -700 against 0; head 1: 0
+    v[0, 1, :, 9] = float("inf")
+    if not new:
+        kc[0, n:], vc[0, n:] = k[0], v[0]
+    out, lse = flash_attn_kvcache_func(q, kc, vc, lens, *((k, v) if new else ()), return_softmax_lse=True)
+    assert torch.isfinite(lse).all() and torch.isfinite(out[..., :9]).all() and torch.isfinite(out[0, 0]).all()
+    assert torch.isnan(out[0, 1:, 0, 9]).all() and torch.isposinf(out[0, 1:, 1, 9]).all()

@@ -29,7 +29,7 @@
 //
 // A row's result depends on what it sees alone: non-finite values of a drafted V row, which the product
 // would multiply by the zero weights of the rows that do not see it, are taken out of the tile and
-// added to the rows that do (a rare path, looked for in steps with drafted keys only).
+// added, times their weight, to the rows that do (a rare path, looked for in steps with drafted keys only).
 // Keys past a sequence's end load as zeros, so no slot behind it reaches a result.  A sequence whose
 // length does not leave room for the drafted tokens, or that names a page outside the cache, gives NaN.
 //
@@ -467,18 +467,30 @@ __global__ void __launch_bounds__(256, groups_per_cu(D, WM)) kv_attn_kernel(cons
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[e] *= inv;
       const int rg = mt * p.tile_rows + rl, t = rg / p.group;
+      const float lse2 = l == 0.f ? kNegInf : m + __log2f(l);
       if (sm_odd[0] | sm_odd[1] | sm_odd[2] | sm_odd[3]) {
+        const u16* q = (const u16*)p.q + (int64_t)bidb * p.q_batch + (int64_t)t * p.q_row +
+                       (int64_t)(kvh * p.group + rg - t * p.group) * p.q_head;
         for (int j = max(len, s0 * kStep); j < min(total, s1 * kStep); ++j) {
-          bool out = false;
-          const u16* v = has_new ? vn + (int64_t)(j - len) * p.vn_row : vc + slot_offset(c, bidb, j, out);
           if (ch * 4 >= c.d || !sees(t, j, mask_byte(t, j))) continue;
+          bool out = false;
+          const int64_t off = has_new ? 0 : slot_offset(c, bidb, j, out);
+          const u16* v = has_new ? vn + (int64_t)(j - len) * p.vn_row : vc + off;
+          const u16* k = has_new ? kn + (int64_t)(j - len) * p.kn_row : kc + off;
+          float weight = -1.f;                     // of the key; (its product with infinity is what adds)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (odd_pair<BF16>(v[ch * 4 + e])) acc[e] += E::to_f32(v[ch * 4 + e]);
+          for (int e = 0; e < 4; ++e) {
+            if (!odd_pair<BF16>(v[ch * 4 + e])) continue;
+            if (weight < 0.f) {
+              float dot = 0.f;
+              for (int i = 0; i < c.d; ++i) dot += E::to_f32(q[i]) * E::to_f32(k[i]);
+              weight = fast_exp2(fmaf(dot, cs, -lse2));
+            }
+            acc[e] += weight * E::to_f32(v[ch * 4 + e]);
+          }
         }
       }
       if (l != l) acc[0] = acc[1] = acc[2] = acc[3] = l;
-      const float lse2 = l == 0.f ? kNegInf : m + __log2f(l);
       if (!whole) {
         const int64_t prow = slot * p.tile_rows + rl;
         if (ch * 4 < c.d) *(f32x4_t*)(p.part_o + prow * c.d + ch * 4) = acc;
