@@ -61,10 +61,12 @@ class QKNormRotary(torch.nn.Module):
         if self._cos is None or self._cos.shape[0] < rows or self._cos.device != device:
             have = 0 if self._cos is None or self._cos.device != device else self._cos.shape[0]
             n = max(rows, 2 * have)
-            inv = self.base ** (-torch.arange(0, self.rotary_dim, 2, device=device, dtype=torch.float64)
-                                / self.rotary_dim)
-            angle = torch.outer(torch.arange(n, device=device, dtype=torch.float64), inv)
-            self._cos, self._sin = angle.cos().float(), angle.sin().float()
+            # (a table made under inference_mode could not be saved for a later backward)
+            with torch.inference_mode(False):
+                inv = self.base ** (-torch.arange(0, self.rotary_dim, 2, device=device, dtype=torch.float64)
+                                    / self.rotary_dim)
+                angle = torch.outer(torch.arange(n, device=device, dtype=torch.float64), inv)
+                self._cos, self._sin = angle.cos().float(), angle.sin().float()
         return self._cos, self._sin
 
     def forward(self, q, k, positions=None, max_position=None):
