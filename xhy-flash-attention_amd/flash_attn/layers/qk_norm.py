@@ -17,6 +17,7 @@ import flash_attn_2_cuda as _ext
 
 __all__ = ["apply_qk_norm_rotary_func", "QKNormRotary"]
 
+
 def apply_qk_norm_rotary_func(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
                               k_weight: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None,
                               sin: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
@@ -45,7 +46,10 @@ class QKNormRotary(torch.nn.Module):
     """The weights of ``apply_qk_norm_rotary_func`` and, with rotary_dim > 0, its cos / sin table.
 
     The table is fp32, computed in fp64 (angles of far positions keep their digits) for as many rows
-    as asked for, and grows by doubling; XPos scaling is not part of it."""
+    as asked for, and grows by doubling; XPos scaling is not part of it.  Tables that were outgrown
+    are kept (all of them together are smaller than the last one): graphs captured with them read them
+    at every replay.  A call in a capture that needs a longer table fills one of its own at every
+    replay; call ``table(rows, device)``, or the step itself, before the capture."""
 
     def __init__(self, headdim: int, rotary_dim: int = 0, base: float = 10000.0, interleaved: bool = False,
                  eps: float = 1e-6, device=None, dtype=None):
@@ -53,21 +57,28 @@ class QKNormRotary(torch.nn.Module):
         self.rotary_dim, self.base, self.interleaved, self.eps = rotary_dim, float(base), interleaved, eps
         self.q_weight = torch.nn.Parameter(torch.ones(headdim, device=device, dtype=dtype))
         self.k_weight = torch.nn.Parameter(torch.ones(headdim, device=device, dtype=dtype))
-        self._cos = self._sin = None
+        self._tables = {}                          # device: its tables, the last one in use
 
     def table(self, rows: int, device) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+        """cos, sin of at least ``rows`` rows on ``device``."""
         if self.rotary_dim == 0:
             return None, None
-        if self._cos is None or self._cos.shape[0] < rows or self._cos.device != device:
-            have = 0 if self._cos is None or self._cos.device != device else self._cos.shape[0]
-            n = max(rows, 2 * have)
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        tables = self._tables.setdefault(device, [])
+        have = tables[-1][0].shape[0] if tables else 0
+        if have < rows:
             # (a table made under inference_mode could not be saved for a later backward)
             with torch.inference_mode(False):
                 inv = self.base ** (-torch.arange(0, self.rotary_dim, 2, device=device, dtype=torch.float64)
                                     / self.rotary_dim)
-                angle = torch.outer(torch.arange(n, device=device, dtype=torch.float64), inv)
-                self._cos, self._sin = angle.cos().float(), angle.sin().float()
-        return self._cos, self._sin
+                angle = torch.outer(torch.arange(max(rows, 2 * have), device=device, dtype=torch.float64), inv)
+                made = angle.cos().float(), angle.sin().float()
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                return made                        # filled by the replays, in the graph's memory: for this call alone
+            tables.append(made)
+        return tables[-1]
 
     def forward(self, q, k, positions=None, max_position=None):
         """q, k as apply_qk_norm_rotary_func; with positions, max_position bounds them (rows of the table)."""
