@@ -81,3 +81,18 @@ def test_table_that_a_capture_fills_serves_no_other_call():
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(out, want))
             assert all(torch.equal(a, b) for a, b in zip(m(q, k, pos, max_position=64), want))
+
+
+@pytest.mark.gpu
+def test_table_made_on_a_busy_stream_serves_others_at_once():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    m = QKNormRotary(64, 64, device="cuda")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(int(2e8))                # the table's kernels wait behind this
+        m.table(1000, "cuda")
+    got = [t.clone() for t in m.table(1000, "cuda")]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, m.table(1000, "cuda")))

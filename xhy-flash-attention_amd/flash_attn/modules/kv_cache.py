@@ -7,8 +7,8 @@
     cache.commit(accepted)                            # of a tree of drafted tokens
     cache.evict(budget, sink=4, recent=256)
 
-Lengths and positions live on the GPU and are updated in place: nothing here synchronises, and a step
-captured into a graph goes on where its last replay stopped.
+Lengths and positions live on the GPU and are updated in place: nothing here synchronises (but a rotary table
+that grows), and a step captured into a graph goes on where its last replay stopped.
 """
 import torch
 
