@@ -23,32 +23,39 @@ class KVCache:
     seqlens: int32 (batch,), the keys held; positions: int32 (batch,), the position of the next token, which
     eviction leaves alone; most: no position is above it (known on the host: it sizes the rotary table.
     Replays of a graph do not count it up: set it to the longest length that they reach before the
-    capture, as a position outside the table gives NaN); attn_weight: fp32 (batch, nheads_k, slots) with
-    track_weight, else None."""
+    capture, as a position outside the table gives NaN); max_position: the longest that a sequence gets,
+    which ``most`` stops at (a commit counts every drafted token into it, as the host does not know how
+    many stay); attn_weight: fp32 (batch, nheads_k, slots) with track_weight, else None."""
 
-    def __init__(self, batch_size, slots, nheads_k, headdim, device=None, dtype=None, track_weight=False):
+    def __init__(self, batch_size, slots, nheads_k, headdim, device=None, dtype=None, track_weight=False,
+                 max_position=None):
         self.k = torch.zeros(batch_size, slots, nheads_k, headdim, device=device, dtype=dtype)
         self.v = torch.zeros_like(self.k)
         self.block_table = None
         self.seqlens = torch.zeros(batch_size, device=device, dtype=torch.int32)
         self.positions = torch.zeros_like(self.seqlens)
-        self.most = 0
+        self.most, self.max_position = 0, max_position
         self.attn_weight = None
         if track_weight:
             self.attn_weight = torch.zeros(batch_size, nheads_k, slots, device=device, dtype=torch.float32)
+
+    def _advance(self, count):
+        self.most += count
+        if self.max_position is not None:
+            self.most = min(self.most, self.max_position)
 
     def accept(self, count):
         """Keeps all ``count`` tokens of the last call."""
         self.seqlens += count
         self.positions += count
-        self.most += count
+        self._advance(count)
 
     def commit(self, accepted):
         """Keeps the accepted ones (bool (batch, seqlen_q)) of the last call's tokens, in their order."""
         seqlens = flash_attn_kvcache_commit_(self.k, self.v, self.seqlens, accepted, self.block_table, self.attn_weight)
         self.positions += seqlens - self.seqlens
         self.seqlens.copy_(seqlens)
-        self.most += accepted.shape[1]
+        self._advance(accepted.shape[1])
 
     def evict(self, budget, sink=0, recent=0):
         """Shrinks sequences of more than ``budget`` keys; returns the slots the kept keys came from."""
