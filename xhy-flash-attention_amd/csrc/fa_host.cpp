@@ -7,6 +7,7 @@
 // kernels stay behind the C ABI of libflash_attn_mi355x.so: bind() is handed the addresses of its entry points
 // by flash_attn_2_cuda, which loads it, so that one library serves both.
 #include <ATen/MemoryOverlap.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -108,7 +109,15 @@ void check_device(const char* op, std::initializer_list<const Tensor*> ts) {
 }
 const Tensor* opt(const OptTensor& t) { return t ? &*t : nullptr; }
 
+// A dual tensor's tangent would be lost without a word: its requires_grad is false.
+void check_no_tangent(const char* op, std::initializer_list<const Tensor*> ts) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : ts)
+    TORCH_CHECK(t == nullptr || !t->_fw_grad(/*level=*/0).defined(), op, ": no forward-mode derivative");
+}
+
 void check_no_grad(std::initializer_list<const Tensor*> ts) {
+  check_no_tangent("kvcache", ts);
   if (!at::GradMode::is_enabled()) return;
   for (const Tensor* t : ts)
     TORCH_CHECK(t == nullptr || !t->requires_grad(), "kvcache: the cache has no backward; call it under torch.no_grad()");
@@ -466,6 +475,7 @@ void check_capture(std::initializer_list<const Tensor*> ts) {
 std::pair<Tensor, Tensor> norm_rotary(const Tensor& q, const Tensor& k, const OptTensor& wq, const OptTensor& wk,
                                       const OptTensor& cos, const OptTensor& sin, const OptTensor& pos, bool interleaved,
                                       double eps, bool inplace) {
+  check_no_tangent("qk_norm_rotary", {&q, &k, opt(wq), opt(wk), opt(cos), opt(sin)});
   if (inplace) check_writable("qk_norm_rotary", {&q, &k});
   check_norm(q, k, wq, wk, cos, sin, pos, eps);
   bool grad = false;
