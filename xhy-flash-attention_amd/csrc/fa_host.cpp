@@ -457,18 +457,23 @@ struct QkNormRotary : torch::autograd::Function<QkNormRotary> {
   }
 };
 
-// A gradient accumulator that an eager graph keeps alive belongs to that graph's stream.  A backward that is
-// being captured would make this stream part of the capture, which torch cannot end: the process does.
+// A gradient accumulator that an eager graph keeps alive belongs to that graph's stream, and a backward that is
+// being captured makes this stream part of the capture.  A side stream joins and is let go at the end; the default
+// stream cannot be captured: torch cannot end such a capture, and the process ends.
 void check_capture(std::initializer_list<const Tensor*> ts) {
-  const auto stream = c10::hip::getCurrentHIPStream((*ts.begin())->device().index());
+  const auto device = (*ts.begin())->device().index();
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+  if (hipStreamIsCapturing(c10::hip::getCurrentHIPStream(device).stream(), &status) != hipSuccess ||
+      status == hipStreamCaptureStatusNone)
+    return;
+  const auto eager = c10::hip::getDefaultHIPStream(device).id();
   for (const Tensor* t : ts) {
     if (t == nullptr || !t->requires_grad() || !t->is_leaf()) continue;
     const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
     const auto of = node ? node->stream() : std::nullopt;
-    TORCH_CHECK(!of || of->id() == stream.id(),
-                "qk_norm_rotary: captured while an eager graph of the same leaves is alive; let go of its outputs first");
+    TORCH_CHECK(!of || of->id() != eager,
+                "qk_norm_rotary: captured while an eager graph of the same leaves, on the default stream, is alive; let go of "
+                "its outputs first, or make it (and a wrapper that holds their accumulators) on a side stream");
   }
 }
 

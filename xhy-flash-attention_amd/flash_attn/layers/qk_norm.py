@@ -36,8 +36,8 @@ def apply_qk_norm_rotary_func(q: torch.Tensor, k: torch.Tensor, q_weight: Option
         inplace: write over q and k (inference: refused when a gradient is asked for).
     Returns q and k normalised and rotated, one rounding from fp32.  Differentiable (once) in q, k and
     the weights; the weights' gradients are summed in a fixed order.  Forward and backward can be captured in
-    a graph; a capture is refused while an eager graph of the same leaves is alive (its gradient accumulators
-    would draw their stream into the capture)."""
+    a graph; a capture is refused while an eager graph of the same leaves that was made on the default stream is
+    alive (its gradient accumulators would draw that stream into the capture)."""
     return _ext.host_module().norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, interleaved, eps,
                                           inplace)
 
