@@ -37,8 +37,10 @@ def flash_attn_kvcache_func(q, k_cache, v_cache, cache_seqlens, k=None, v=None, 
             seen.  A drafted token that no row sees may hold anything.
         softmax_scale: default 1 / sqrt(headdim).
         attn_weight: fp32 (batch, nheads_k, slots), optional: every key's entry grows by the sum of its
-            probabilities over the rows of the query heads that share the kv head.  With fewer columns
-            than the cache has slots, sequences have room for as many keys (in the other calls too).
+            probabilities over the rows of the query heads that share the kv head, the drafted tokens' entries
+            among them: they should hold 0 before (commit and eviction leave it so; after a call whose tokens
+            are not kept, KVCache.clear_drafts does).  With fewer columns than the cache has slots, sequences
+            have room for as many keys (in the other calls too).
         return_softmax_lse: also return the log-sum-exp of the scaled scores, fp32 (batch, nheads, seqlen_q).
     cache_seqlens is not changed (flash_attn_kvcache_commit_ gives the new lengths).  A row that sees
     no key gives 0 and +inf.  A sequence whose length leaves no room for the drafted tokens, or that

@@ -38,6 +38,14 @@ class KVCache:
         self.attn_weight = None
         if track_weight:
             self.attn_weight = torch.zeros(batch_size, nheads_k, slots, device=device, dtype=torch.float32)
+            self._slot = torch.arange(slots, device=device, dtype=torch.int32)
+
+    def clear_drafts(self):
+        """Before a call: the weights of the slots behind the keys held become 0.  A call whose tokens were not
+        kept has left theirs there, and the next call adds to them (what its tokens gave to the keys
+        held stays: those were looked at)."""
+        if self.attn_weight is not None:
+            self.attn_weight.masked_fill_((self._slot >= self.seqlens[:, None])[:, None], 0.0)
 
     def _advance(self, count):
         self.most += count

@@ -235,6 +235,7 @@ class MHA(nn.Module):
                 depth = torch.arange(x.shape[1], device=x.device, dtype=torch.int32)
             q, k = self.qk_norm(q, k, (cache.positions[:, None] + depth).to(torch.int32).expand(x.shape[:2]),
                                 cache.most + x.shape[1])
+        cache.clear_drafts()
         context = flash_attn_kvcache_func(q, cache.k, cache.v, cache.seqlens, k=k, v=v, block_table=cache.block_table,
                                           tree_mask=tree_mask, softmax_scale=self.inner_attn.softmax_scale,
                                           attn_weight=cache.attn_weight)
