@@ -106,3 +106,41 @@ def test_tokens_that_were_not_kept_leave_no_weight(captured):
         err = (a.attn_weight[:, :, 10:] - b.attn_weight[:, :, 10:]).abs()
         assert (err <= 1.03 * 2 * ds * b.attn_weight[:, :, 10:]).all()
     assert a.seqlens.tolist() == [13, 13] and (a.attn_weight[:, :, 13:] == 0).all()
+
+
+@pytest.mark.parametrize("paged", [False, True])
+def test_accept_leaves_a_sequence_without_room(paged):
+    """The call stored nothing for it: its length stays one that eviction and commit take."""
+    c = KVCache(3, 8 if paged else 32, 1, 8)
+    if paged:
+        c.block_table = torch.zeros(3, 4, dtype=torch.int32)
+    c.seqlens.copy_(torch.tensor([0, 28, 29], dtype=torch.int32))
+    c.positions.copy_(torch.tensor([0, 50, 51], dtype=torch.int32))
+    c.accept(4)
+    assert c.seqlens.tolist() == [4, 32, 29] and c.positions.tolist() == [4, 54, 51]
+    assert c.seqlens.dtype == c.positions.dtype == torch.int32
+    c.attn_weight = torch.zeros(3, 1, 10)          # fewer columns than slots
+    c.accept(6)
+    assert c.seqlens.tolist() == [10, 32, 29]
+
+
+@pytest.mark.gpu
+def test_a_full_cache_goes_on_after_eviction():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    from flash_attn.modules.mha import MHA
+    torch.manual_seed(0)
+    m = MHA(64, 2, causal=True, device="cuda", dtype=torch.float16)
+    x = torch.randn(2, 16, 64, device="cuda", dtype=torch.float16)
+    with torch.no_grad():
+        c = KVCache(2, 16, 2, 32, device="cuda", dtype=torch.float16, track_weight=True)
+        m(x[:, :15], kv_cache=c)
+        c.accept(15)
+        assert torch.isnan(m(x[:, :3], kv_cache=c)).all()
+        c.accept(3)                                # nothing was stored
+        assert c.seqlens.tolist() == [15, 15]
+        kept = c.evict(8, sink=2, recent=2)
+        assert c.seqlens.tolist() == [8, 8] and (kept >= 0).all()
+        assert torch.isfinite(m(x[:, :3], kv_cache=c)).all()
+        c.accept(3)
+        assert c.seqlens.tolist() == [11, 11] and c.positions.tolist() == [18, 18]

@@ -52,10 +52,15 @@ class KVCache:
         if self.max_position is not None:
             self.most = min(self.most, self.max_position)
 
+    def _room(self):
+        slots = self.k.shape[1] * (1 if self.block_table is None else self.block_table.shape[1])
+        return slots if self.attn_weight is None else min(slots, self.attn_weight.shape[2])
+
     def accept(self, count):
-        """Keeps all ``count`` tokens of the last call."""
-        self.seqlens += count
-        self.positions += count
+        """Keeps all ``count`` tokens of the last call; a sequence that had no room for them stays as it is."""
+        kept = self.seqlens <= self._room() - count
+        self.seqlens.add_(kept, alpha=count)
+        self.positions.add_(kept, alpha=count)
         self._advance(count)
 
     def commit(self, accepted):
