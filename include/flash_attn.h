@@ -462,7 +462,8 @@ size_t flash_attn_qk_norm_rotary_workspace(int head_size);
  * (num_pages, page_size, num_heads_k, head_size); cache_strides = {sequence or page, row, head} in
  * ELEMENTS, the same for both, multiples of 8 on 16-byte bases; block_table: int32, row stride
  * block_table_stride, entry [i][j / page_size] is the page of key j of sequence i; page_size 0: none.
- * `slots` is the number of keys a sequence has room for (with pages at most entries x page_size).
+ * `slots` is the number of keys a sequence has room for (with pages at most entries x page_size; an eviction's
+ * budget and slots are at most 2^31 - 2^16).
  * cache_seqlens: int32 (batch), the keys each sequence holds.  head_size % 8 == 0, <= 256.
  * No entry point reads or writes outside the cache whatever cache_seqlens and block_table hold.
  *

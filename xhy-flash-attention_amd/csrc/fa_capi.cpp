@@ -495,7 +495,7 @@ fa::KvCache make_cache(void* k_cache, void* v_cache, const int32_t* lens, const 
                        const int64_t* strides, int b, int slots, int hk, int d, int page, int num_pages) {
   check_device();
   FA_CHECK(k_cache && v_cache && lens && strides);
-  FA_CHECK(b > 0 && slots > 0 && hk > 0);
+  FA_CHECK(b > 0 && slots > 0 && slots <= fa::kKvMaxSlots && hk > 0);
   FA_CHECK(d > 0 && d % 8 == 0 && d <= 256);
   FA_CHECK((table != nullptr) == (page > 0));
   if (table != nullptr) FA_CHECK(num_pages > 0);
@@ -512,7 +512,7 @@ fa::KvCache make_cache(void* k_cache, void* v_cache, const int32_t* lens, const 
 
 void attn_sizes(fa::KvAttnParams& p, int b, int sq, int slots, int h, int hk, int d) {
   FA_CHECK(b > 0 && sq > 0 && h > 0 && hk > 0 && h % hk == 0);
-  FA_CHECK((int64_t)sq * (h / hk) <= (1 << 20) && slots <= 0x7fffff00);
+  FA_CHECK((int64_t)sq * (h / hk) <= (1 << 20) && slots <= fa::kKvMaxSlots);
   FA_CHECK(d > 0 && d <= 256);
   p.c.b = b; p.c.hk = hk; p.c.d = d; p.c.slots = slots;
   p.h = h; p.sq = sq; p.group = h / hk; p.rows = sq * p.group;
@@ -664,7 +664,7 @@ bool flash_attn_kvcache_evict(void* const k_cache, void* const v_cache, const in
                    num_heads_k, head_size, page_size, num_pages);
   FA_CHECK(attn_weight && seqlens_out && attn_weight_out && kept && workspace);
   FA_CHECK(attn_weight_strides && attn_weight_out_strides && attn_weight != attn_weight_out);
-  FA_CHECK(budget > 0 && sink >= 0 && recent >= 0 && (int64_t)sink + recent <= budget);
+  FA_CHECK(budget > 0 && budget <= fa::kKvMaxSlots && sink >= 0 && recent >= 0 && (int64_t)sink + recent <= budget);
   FA_CHECK(batch_size <= 65535);
   p.weight = attn_weight; p.w_batch = attn_weight_strides[0]; p.w_head = attn_weight_strides[1];
   p.weight_out = attn_weight_out; p.wo_batch = attn_weight_out_strides[0]; p.wo_head = attn_weight_out_strides[1];

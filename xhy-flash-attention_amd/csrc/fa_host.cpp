@@ -126,6 +126,7 @@ void check_no_grad(std::initializer_list<const Tensor*> ts) {
 // ------------------------------------------------------------------------------------------------
 // key/value cache
 // ------------------------------------------------------------------------------------------------
+constexpr int64_t kMaxSlots = 0x7fff0000;   // (the C ABI's limit: the kernels' int counters run past the last slot)
 struct Cache {
   int64_t b, slots, page = 0, pages = 0, hk, d, table_stride = 0;
   Strides strides;
@@ -159,7 +160,7 @@ struct Cache {
       slots = table->size(1) * page;
       table_stride = table->stride(0);
     }
-    TORCH_CHECK(slots < 0x7fffff00 && page < 0x7fffff00 && pages < 0x7fffff00 && hk < (1 << 24),
+    TORCH_CHECK(slots <= kMaxSlots && page <= kMaxSlots && pages <= kMaxSlots && hk < (1 << 24),
                 "kvcache: too many slots");
   }
   // weights of fewer columns than there are slots limit the room of a sequence
@@ -276,8 +277,8 @@ std::tuple<Tensor, Tensor, Tensor> evict(const Tensor& k_cache, const Tensor& v_
                                          const Tensor& weight, int64_t budget, int64_t sink, int64_t recent,
                                          const OptTensor& table) {
   Cache c(k_cache, v_cache, lens, table);
-  TORCH_CHECK(budget > 0 && budget < 0x7fffff00 && sink >= 0 && recent >= 0 && sink <= budget && recent <= budget - sink,
-              "kvcache: budget must be positive and at least sink + recent");
+  TORCH_CHECK(budget > 0 && budget <= kMaxSlots && sink >= 0 && recent >= 0 && sink <= budget && recent <= budget - sink,
+              "kvcache: budget must be positive, at least sink + recent and at most 2^31 - 2^16");
   TORCH_CHECK(c.b <= 65535, "kvcache: batch size must be at most 65535");
   c.limit(weight);
   check_no_grad({&k_cache, &v_cache, &weight});

@@ -167,6 +167,7 @@ __global__ void __launch_bounds__(256, groups_per_cu(D, WM)) kv_attn_kernel(cons
   const int oct = (blockIdx.x >> 3) / units, unit = (blockIdx.x >> 3) - oct * units;
   const int share = oct * 8 + (blockIdx.x & 7);
   const int mt = unit / c.hk, kvh = unit - mt * c.hk;
+  if (share >= p.shares) return;                   // (of the last eight)
   const Shares sh(p, lane);
   int at = share * sh.share;
   const int end = min(sh.total, at + sh.share);
@@ -741,7 +742,7 @@ void kv_attn_plan(KvAttnParams& p) {
   p.m_tiles = (p.rows + per - 1) / per;
   p.tile_rows = std::min(p.rows, ((p.rows + p.m_tiles - 1) / p.m_tiles + 31) / 32 * 32);
   const int64_t units = (int64_t)p.c.hk * p.m_tiles, steps = (int64_t)p.c.b * ((p.c.slots + kStep - 1) / kStep);
-  if (steps > 0x7fffffff || units > 0xffffff) throw std::runtime_error("kvcache attention: too many keys for one launch");
+  if (steps > 0x7fff0000 || units > 0xffffff) throw std::runtime_error("kvcache attention: too many keys for one launch");
   const int dd = p.c.d <= 64 ? 64 : p.c.d <= 128 ? 128 : 256;
   const int64_t resident = 256 * groups_per_cu(dd, per / 32);
   p.shares = (int)std::min(steps, units <= resident / 4 ? resident / units : (4 * resident + units - 1) / units);

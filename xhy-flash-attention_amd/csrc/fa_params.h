@@ -175,6 +175,9 @@ struct QkNormParams {
 // Key/value cache (fa_kvcache.hip).  The cache is (b, slots, hk, d) (table == nullptr) or pages of
 // (num_pages, page, hk, d) with table (b, blocks) naming the page of each block of `page` keys; K and V
 // share their strides.  Sequence i holds lens[i] keys; sq drafted tokens follow at slots lens[i] ...
+// The kernels walk slots, and the places of an eviction's budget, with int counters that run past the last one by
+// up to a chunk of 32k: no more slots than leave room for that.
+constexpr int kKvMaxSlots = 0x7fff0000;
 struct KvCache {
   void* k; void* v;
   const int* table;
