@@ -28,3 +28,26 @@ def test_slots_that_the_counters_would_run_over():
             flash_attn_kvcache_func(q, k, v, lens, block_table=table)
     with pytest.raises(RuntimeError, match="too many slots"):
         flash_attn_kvcache_evict_(k, v, lens, torch.zeros(1, 1, 50), 10, block_table=torch.zeros(1, (1 << 16) - 1, dtype=torch.int32))
+
+
+def test_a_prompt_needs_no_workspace():
+    """Row tiles that fill the chip by themselves walk all keys: no sequence is cut, nothing is left to merge."""
+    import ctypes
+    import flash_attn_2_cuda as m
+    w = m._lib.flash_attn_kvcache_workspace
+    w.argtypes, w.restype = [ctypes.c_int] * 6 + [ctypes.c_bool], ctypes.c_size_t
+    assert w(1, 8192, 16384, 32, 8, 128, False) == 0
+    assert w(4, 4096, 4096, 64, 64, 64, True) == 0
+    assert w(1, 48, 16384, 32, 8, 128, False) > 0   # a tree is cut
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,weight", [(64, False), (128, True)])
+def test_a_prompt_that_is_not_cut(d, weight):
+    """Enough heads and tokens for one share: every sequence is written at once, weights included."""
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    import flash_attn_2_cuda as m
+    from test_kvcache_gpu import _run
+    assert m._lib.flash_attn_kvcache_workspace(2, 1100, 1200, 256, 256, d, weight) == 0
+    _run(2, 1100, 256, 256, d, [0, 37], torch.bfloat16, 0, weight=weight, slack=63)

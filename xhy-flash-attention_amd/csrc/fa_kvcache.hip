@@ -756,8 +756,8 @@ static bool store_scores(const KvAttnParams& p) {
   return p.weight != nullptr && p.rows <= kScoreRows && 4 * p.rows <= p.c.d && p.rows * p.score_pitch < (1 << 29);
 }
 
-// a sequence of one step is never cut
-static bool may_cut(const KvAttnParams& p) { return p.c.slots > kStep; }
+// a sequence of one step is never cut, nor any where all steps are one share (a prompt's row tiles fill the chip)
+static bool may_cut(const KvAttnParams& p) { return p.c.slots > kStep && p.shares > 1; }
 
 static size_t part_floats(const KvAttnParams& p) {
   return may_cut(p) ? ((size_t)p.shares * p.c.hk * p.m_tiles * 2 * p.tile_rows * (p.c.d + 1) + 3) / 4 * 4 : 0;
