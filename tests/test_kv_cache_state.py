@@ -144,3 +144,12 @@ def test_a_full_cache_goes_on_after_eviction():
         assert torch.isfinite(m(x[:, :3], kv_cache=c)).all()
         c.accept(3)
         assert c.seqlens.tolist() == [11, 11] and c.positions.tolist() == [18, 18]
+
+
+@pytest.mark.parametrize("columns", [10, 6, 14])
+def test_clear_drafts_of_weights_that_were_put_in(columns):
+    c = KVCache(2, 10, 2, 8)
+    c.attn_weight = torch.ones(2, 2, columns)
+    c.seqlens.copy_(torch.tensor([3, 6], dtype=torch.int32))
+    c.clear_drafts()
+    assert c.attn_weight.sum(-1).tolist() == [[3, 3], [6, 6]]

@@ -35,17 +35,21 @@ class KVCache:
         self.seqlens = torch.zeros(batch_size, device=device, dtype=torch.int32)
         self.positions = torch.zeros_like(self.seqlens)
         self.most, self.max_position = 0, max_position
+        self._slot = torch.arange(slots, device=device, dtype=torch.int32)
         self.attn_weight = None
         if track_weight:
             self.attn_weight = torch.zeros(batch_size, nheads_k, slots, device=device, dtype=torch.float32)
-            self._slot = torch.arange(slots, device=device, dtype=torch.int32)
 
     def clear_drafts(self):
         """Before a call: the weights of the slots behind the keys held become 0.  A call whose tokens were not
         kept has left theirs there, and the next call adds to them (what its tokens gave to the keys
         held stays: those were looked at)."""
-        if self.attn_weight is not None:
-            self.attn_weight.masked_fill_((self._slot >= self.seqlens[:, None])[:, None], 0.0)
+        if self.attn_weight is None:
+            return
+        slot, columns = self._slot, self.attn_weight.shape[2]
+        if slot.numel() != columns:                # weights of the caller's own
+            slot = torch.arange(columns, device=slot.device, dtype=torch.int32)
+        self.attn_weight.masked_fill_((slot >= self.seqlens[:, None])[:, None], 0.0)
 
     def _advance(self, count):
         self.most += count
