@@ -287,7 +287,10 @@ std::tuple<Tensor, Tensor, Tensor> evict(const Tensor& k_cache, const Tensor& v_
   const c10::DeviceGuard guard(k_cache.device());
   Tensor out = at::empty_like(lens);
   Tensor weight_out = at::empty({c.b, c.hk, weight.size(2)}, weight.options());
-  if (weight.size(2) > c.slots) weight_out.slice(2, c.slots).copy_(weight.slice(2, c.slots));
+  if (weight.size(2) > c.slots) {   // columns that no slot belongs to: 0 behind a sequence's keys as well
+    const Tensor held = lens.ge(0).logical_and_(lens.le(c.slots)).unsqueeze(1).unsqueeze(2);
+    weight_out.slice(2, c.slots).copy_(weight.slice(2, c.slots).masked_fill(held, 0.0));
+  }
   Tensor kept = at::empty({c.b, c.hk, budget}, lens.options());
   Tensor work = at::empty({c.b * c.hk}, lens.options());
   const int64_t ws[2] = {weight.stride(0), weight.stride(1)}, wo[2] = {weight_out.stride(0), weight_out.stride(1)};
