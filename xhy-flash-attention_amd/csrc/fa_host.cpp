@@ -13,7 +13,9 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
+#include <functional>
 #include <optional>
 #include <string>
 #include <unordered_map>
@@ -81,6 +83,39 @@ void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 Tensor vec_ok(const Tensor& t) { return aligned(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+// Whether two views of one storage share an element: their offsets differ by sum x_i stride_i for some x_i in
+// [1 - size_i of b, size_i of a - 1].  Looked for from the largest stride down, where what the smaller ones reach
+// leaves one or two x_i to try.  Views of unlike strides stay undecided (false).
+bool share_elements(const Tensor& a, const Tensor& b) {
+  if (!a.storage().is_alias_of(b.storage()) || a.numel() == 0 || b.numel() == 0) return false;
+  if (a.dim() != b.dim() || a.scalar_type() != b.scalar_type()) return false;
+  struct Dim { int64_t stride, lo, hi; };
+  Dim dims[8];
+  int n = 0;
+  for (int64_t i = 0; i < a.dim(); ++i) {
+    if (a.size(i) == 1 && b.size(i) == 1) continue;
+    if (n == 8 || (a.size(i) > 1 && b.size(i) > 1 && a.stride(i) != b.stride(i))) return false;
+    dims[n++] = {a.size(i) > 1 ? a.stride(i) : b.stride(i), 1 - b.size(i), a.size(i) - 1};
+  }
+  std::sort(dims, dims + n, [](const Dim& x, const Dim& y) { return x.stride > y.stride; });
+  int64_t low[9] = {}, high[9] = {};   // what dims i .. reach
+  for (int i = n; i-- > 0;) {
+    low[i] = low[i + 1] + dims[i].stride * dims[i].lo;
+    high[i] = high[i + 1] + dims[i].stride * dims[i].hi;
+  }
+  int tries = 256;                     // (strides that do not nest could ask for more)
+  const std::function<bool(int, int64_t)> reach = [&](int i, int64_t rest) {
+    if (rest < low[i] || rest > high[i] || --tries < 0) return false;
+    if (i == n) return rest == 0;
+    if (dims[i].stride == 0) return reach(i + 1, rest);
+    const int64_t mid = rest / dims[i].stride;
+    for (int64_t x = std::max(dims[i].lo, mid - 1); x <= std::min(dims[i].hi, mid + 1); ++x)
+      if (reach(i + 1, rest - x * dims[i].stride)) return true;
+    return false;
+  };
+  return reach(0, b.storage_offset() - a.storage_offset());
+}
+
 // t is written: an expanded tensor, or two that share elements, would be by several rows at once
 void check_writable(const char* op, std::initializer_list<const Tensor*> ts) {
   for (const Tensor* a : ts) {
@@ -91,7 +126,7 @@ void check_writable(const char* op, std::initializer_list<const Tensor*> ts) {
       if (b == nullptr) continue;
       const auto overlap = at::get_overlap_status(*a, *b);
       TORCH_CHECK(a->unsafeGetTensorImpl() != b->unsafeGetTensorImpl() && overlap != at::MemOverlapStatus::Full &&
-                      overlap != at::MemOverlapStatus::Partial,
+                      overlap != at::MemOverlapStatus::Partial && !share_elements(*a, *b),
                   op, ": written tensors must not share memory");
     }
   }
