@@ -473,7 +473,8 @@ size_t flash_attn_qk_norm_rotary_workspace(int head_size);
  * already) are also stored into those slots.  out (batch, seqlen_q, num_heads, head_size);
  * softmax_lse (batch, num_heads, seqlen_q) fp32; rows that see no key give out = 0, LSE = +inf.
  * attn_weight (fp32, optional): [i][kv head][key] += the sum over the rows of that kv head's query
- * heads of exp(softmax_scale q.k - LSE), strides {batch, head}.  A sequence whose length leaves no
+ * heads of exp(softmax_scale q.k - LSE), strides {batch, head}; the drafted keys' entries grow too, so they
+ * should hold 0 before.  A sequence whose length leaves no
  * room for the drafted tokens gives NaN and stores nothing; a page outside the cache gives NaN.
  * strides arguments: {batch, row, head}.  workspace: flash_attn_kvcache_workspace(...) bytes, 16-byte
  * aligned (attn_weight: whether the call has one). */

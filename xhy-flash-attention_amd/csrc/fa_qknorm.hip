@@ -15,8 +15,8 @@
 //   * a lane keeps one token's angles in registers for up to NH heads of it, and issues all of their
 //     row loads before the first use;
 //   * W = 8 (16-byte pieces) where strides, rotary_dim and the tables allow it; W = 1 takes every
-//     other shape with 64 lanes per row (4 x 8192 tokens, 32 + 8 heads of 128: W = 1 takes 339 us forward
-//     and 914 backward against 124 and 205);
+//     other shape with 64 lanes per row (4 x 8192 tokens, 32 + 8 heads of 128, rotary_dim 24, 40 or 54: 328 us
+//     forward and 1005 backward against 125 and 205);
 //   * the backward is one round of resident workgroups over the rows, each with its partial of dw.
 // Measured on those 4 x 8192 tokens, bf16: forward 124 us (0.67 GB, 5.4 TB/s, what a copy reaches),
 // backward 205 + 6 us (1.0 GB, 4.8 TB/s); 16 tokens: 4.0 us, a launch.
