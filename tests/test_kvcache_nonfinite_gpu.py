@@ -77,3 +77,31 @@ def test_a_weight_of_zero_makes_infinity_nan(n, new, sq):
     out, lse = flash_attn_kvcache_func(q, kc, vc, lens, *((k, v) if new else ()), return_softmax_lse=True)
     assert torch.isfinite(lse).all() and torch.isfinite(out[..., :9]).all() and torch.isfinite(out[0, 0]).all()
     assert torch.isnan(out[0, 1:, 0, 9]).all() and torch.isposinf(out[0, 1:, 1, 9]).all()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_many_nonfinite_drafts_do_not_hold_the_gpu(value, d):
+    """A prompt with a V channel that overflowed in every token: what is taken out and added again one key after
+    another stays a matter of milliseconds."""
+    from flash_attn import flash_attn_kvcache_func
+    torch.manual_seed(0)
+    sq, h, hk = 1024, 4, 2
+    lens = torch.tensor([5], device=DEV, dtype=torch.int32)
+    kc, vc, _ = _cache(1, 5 + sq, hk, d, torch.float16, 0)
+    q = 0.1 * torch.randn(1, sq, h, d, device=DEV).half()
+    k, v = (torch.randn(1, sq, hk, d, device=DEV).half() for _ in range(2))
+    clean = flash_attn_kvcache_func(q, kc, vc, lens, k, v)
+    v[..., 3], v[:, :, 1, 40:] = value, value
+    times = []
+    for _ in range(2):
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        start.record()
+        out = flash_attn_kvcache_func(q, kc, vc, lens, k, v)
+        end.record()
+        torch.cuda.synchronize()
+        times.append(start.elapsed_time(end))
+    assert min(times) < 200, times
+    want = clean.clone()
+    want[..., 3], want[:, :, h // 2:, 40:] = value, value
+    torch.testing.assert_close(out, want, rtol=0, atol=0, equal_nan=True)

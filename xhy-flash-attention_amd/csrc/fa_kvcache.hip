@@ -29,7 +29,8 @@
 //
 // A row's result depends on what it sees alone: non-finite values of a drafted V row, which the product
 // would multiply by the zero weights of the rows that do not see it, are taken out of the tile and
-// added, times their weight, to the rows that do (a rare path, looked for in steps with drafted keys only).
+// added, times their weight, to the rows that do (a rare path, looked for in steps with drafted keys only, and
+// gone only where some row of the unit does not see some key: a prompt's rows around the diagonal).
 // Keys past a sequence's end load as zeros, so no slot behind it reaches a result.  A sequence whose
 // length does not leave room for the drafted tokens, or that names a page outside the cache, gives NaN.
 //
@@ -206,6 +207,9 @@ __global__ void __launch_bounds__(256, groups_per_cu(D, WM)) kv_attn_kernel(cons
     const u16* kn = (const u16*)p.k_new + (int64_t)bidb * p.kn_batch + (int64_t)kvh * p.kn_head;
     const u16* vn = (const u16*)p.v_new + (int64_t)bidb * p.vn_batch + (int64_t)kvh * p.vn_head;
     bool bad = false, found_odd = false;
+    // The first of the 32-key tiles that some row of the unit does not see whole (without a mask: its first token
+    // sees the drafted keys up to itself)
+    const int split = p.mask != nullptr ? len & ~31 : (max(0, len + mt * p.tile_rows / p.group + 1) & ~31);
 
     const int row_off = chunk_ok ? (St::row(0, lane) * (int)c.row + chunk) * 2 : (1 << 31);
     constexpr int DEPTH = steps_ahead(D, WM);
@@ -282,7 +286,7 @@ __global__ void __launch_bounds__(256, groups_per_cu(D, WM)) kv_attn_kernel(cons
           *(u32x4_t*)(mine + off) = kx;
           *(u32x4_t*)(mine + TILE + off) = vx;
         }
-        if (j0 + 32 > len && __any(odd != 0)) {    // (rare: through LDS, sparing the registers)
+        if (j0 >= split && __any(odd != 0)) {      // (rare: through LDS, sparing the registers)
           found_odd = true;
 #pragma unroll 1
           for (int i = lane; i < D / 32 * 256; i += 64) {   // 256 pairs of words a panel, 8 a row
@@ -472,25 +476,36 @@ __global__ void __launch_bounds__(256, groups_per_cu(D, WM)) kv_attn_kernel(cons
       const int rg = mt * p.tile_rows + rl, t = rg / p.group;
       const float lse2 = l == 0.f ? kNegInf : m + __log2f(l);
       if (sm_odd[0] | sm_odd[1] | sm_odd[2] | sm_odd[3]) {
+        // the CH lanes of a row go through its drafted keys together, each with 4 columns of V and of the score
+        const bool in = ch * 4 < c.d;
         const u16* q = (const u16*)p.q + (int64_t)bidb * p.q_batch + (int64_t)t * p.q_row +
                        (int64_t)(kvh * p.group + rg - t * p.group) * p.q_head;
-        for (int j = max(len, s0 * kStep); j < min(total, s1 * kStep); ++j) {
-          if (ch * 4 >= c.d || !sees(t, j, mask_byte(t, j))) continue;
+        auto four = [&](const u16* row) { return in ? *(const u32x2_t*)(row + ch * 4) : u32x2_t{0u, 0u}; };
+        auto elt = [](u32x2_t x, int e) { return E::to_f32((u16)(x[e >> 1] >> (e & 1) * 16)); };
+        auto of_row = [&](bool x) { return __ballot(x) >> (lane & ~(CH - 1)) & (~0ull >> (64 - CH)); };
+        const u32x2_t qx = four(q);
+        const int last = min(p.mask == nullptr ? min(total, len + t + 1) : total, s1 * kStep);
+        for (int j = max(max(len, split), s0 * kStep); j < last; ++j) {
+          if (!sees(t, j, mask_byte(t, j))) continue;
           bool out = false;
           const int64_t off = has_new ? 0 : slot_offset(c, bidb, j, out);
-          const u16* v = has_new ? vn + (int64_t)(j - len) * p.vn_row : vc + off;
-          const u16* k = has_new ? kn + (int64_t)(j - len) * p.kn_row : kc + off;
-          float weight = -1.f;                     // of the key; (its product with infinity is what adds)
+          const u32x2_t v = four(has_new ? vn + (int64_t)(j - len) * p.vn_row : vc + off);
+          const unsigned odd[2] = {odd_pair<BF16>(v[0]), odd_pair<BF16>(v[1])};
+          if (of_row((odd[0] | odd[1]) != 0) == 0) continue;
+          const u32x2_t k = four(has_new ? kn + (int64_t)(j - len) * p.kn_row : kc + off);
+          float dot = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dot += elt(qx, e) * elt(k, e);
+#pragma unroll
+          for (int x = 1; x < CH; x <<= 1) dot += __shfl_xor(dot, x);
+          const float weight = fast_exp2(fmaf(dot, cs, -lse2));
+          bool done = true;                        // (NaN already: no key changes that)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            if (!odd_pair<BF16>(v[ch * 4 + e])) continue;
-            if (weight < 0.f) {
-              float dot = 0.f;
-              for (int i = 0; i < c.d; ++i) dot += E::to_f32(q[i]) * E::to_f32(k[i]);
-              weight = fast_exp2(fmaf(dot, cs, -lse2));
-            }
-            acc[e] += weight * E::to_f32(v[ch * 4 + e]);
+            if (odd[e >> 1] >> (e & 1) * 16 & 1) acc[e] += weight * elt(v, e);
+            done = done && acc[e] != acc[e];
           }
+          if (of_row(in && !done) == 0) break;
         }
       }
       if (l != l) acc[0] = acc[1] = acc[2] = acc[3] = l;
