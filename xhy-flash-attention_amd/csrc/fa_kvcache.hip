@@ -29,8 +29,8 @@
 //
 // A row's result depends on what it sees alone: non-finite values of a drafted V row, which the product
 // would multiply by the zero weights of the rows that do not see it, are taken out of the tile and
-// added, times their weight, to the rows that do (a rare path, looked for in steps with drafted keys only, and
-// gone only where some row of the unit does not see some key: a prompt's rows around the diagonal).
+// added, times their weight, to the rows that do (a rare path, looked for in steps with drafted keys, and gone
+// for keys that some row of the unit does not see: a tree's, or those around a prompt's diagonal).
 // Keys past a sequence's end load as zeros, so no slot behind it reaches a result.  A sequence whose
 // length does not leave room for the drafted tokens, or that names a page outside the cache, gives NaN.
 //
@@ -135,6 +135,12 @@ __device__ inline unsigned odd_pair(unsigned u) {
   return ((u & m) == m ? 0xffffu : 0u) | ((u & (m << 16)) == (m << 16) ? 0xffff0000u : 0u);
 }
 
+// The first drafted key that some row of the unit does not see, rounded down to a tile of 32 keys (without a mask
+// the unit's first token sees the drafted keys up to itself)
+__device__ inline int first_hidden(const KvAttnParams& p, int len, int mt) {
+  return max(len, p.mask != nullptr ? len : (len + mt * p.tile_rows / p.group + 1) & ~31);
+}
+
 // Workgroups a CU, and steps in flight.  Few rows: one workgroup of up to 512 registers a wave and two
 // steps; row tiles that are bound by the softmax and the products want two waves a SIMD instead.  (8
 // sequences of 26k keys, 32 / 8 heads of 128: 205 us, against 218 with two workgroups of one step each, and
@@ -207,9 +213,6 @@ __global__ void __launch_bounds__(256, groups_per_cu(D, WM)) kv_attn_kernel(cons
     const u16* kn = (const u16*)p.k_new + (int64_t)bidb * p.kn_batch + (int64_t)kvh * p.kn_head;
     const u16* vn = (const u16*)p.v_new + (int64_t)bidb * p.vn_batch + (int64_t)kvh * p.vn_head;
     bool bad = false, found_odd = false;
-    // The first of the 32-key tiles that some row of the unit does not see whole (without a mask: its first token
-    // sees the drafted keys up to itself)
-    const int split = p.mask != nullptr ? len & ~31 : (max(0, len + mt * p.tile_rows / p.group + 1) & ~31);
 
     const int row_off = chunk_ok ? (St::row(0, lane) * (int)c.row + chunk) * 2 : (1 << 31);
     constexpr int DEPTH = steps_ahead(D, WM);
@@ -275,22 +278,22 @@ __global__ void __launch_bounds__(256, groups_per_cu(D, WM)) kv_attn_kernel(cons
         for (int i = 0; i < St::NI; ++i) {
           const int off = panel_off(St::row(i, ln), St::chunk(ln), NR);
           const unsigned keep = chunk_ok && j0 + St::row(i, ln) < total ? ~0u : 0u;
-          const unsigned drafted = j0 + St::row(i, ln) >= len ? ~0u : 0u;
           u32x4_t kx, vx;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             kx[e] = st.k[i][e] & keep;
             vx[e] = st.v[i][e] & keep;
-            odd |= odd_pair<BF16>(vx[e]) & drafted;
+            odd |= odd_pair<BF16>(vx[e]);
           }
           *(u32x4_t*)(mine + off) = kx;
           *(u32x4_t*)(mine + TILE + off) = vx;
         }
-        if (j0 >= split && __any(odd != 0)) {      // (rare: through LDS, sparing the registers)
+        if (__builtin_expect(j0 + 32 > len && __any(odd != 0), 0)) {    // (rare: through LDS, sparing the registers)
           found_odd = true;
+          const int first = first_hidden(p, len, opaque(mt));
 #pragma unroll 1
           for (int i = lane; i < D / 32 * 256; i += 64) {   // 256 pairs of words a panel, 8 a row
-            if (j0 + ((i & 255) >> 3) < len) continue;      // (cached: every row sees it)
+            if (j0 + ((i & 255) >> 3) < first) continue;
             u32x2_t* const x = (u32x2_t*)(mine + TILE + (i >> 8) * NR * 64) + (i & 255);
             *x = u32x2_t{(*x)[0] & ~odd_pair<BF16>((*x)[0]), (*x)[1] & ~odd_pair<BF16>((*x)[1])};
           }
@@ -475,17 +478,21 @@ __global__ void __launch_bounds__(256, groups_per_cu(D, WM)) kv_attn_kernel(cons
       for (int e = 0; e < 4; ++e) acc[e] *= inv;
       const int rg = mt * p.tile_rows + rl, t = rg / p.group;
       const float lse2 = l == 0.f ? kNegInf : m + __log2f(l);
-      if (sm_odd[0] | sm_odd[1] | sm_odd[2] | sm_odd[3]) {
-        // the CH lanes of a row go through its drafted keys together, each with 4 columns of V and of the score
-        const bool in = ch * 4 < c.d;
+      if (__builtin_expect(sm_odd[0] | sm_odd[1] | sm_odd[2] | sm_odd[3], 0)) {
+        // The CH lanes of a row go through its drafted keys together, each with 4 columns of V and of the score.
+        // (opaque, unroll 1: else lane constants are made before the loop over the steps and spill there: d = 256
+        // decoding 525 us, 440 so)
+        const int col = opaque(ch) * 4;
+        const bool in = col < c.d;
         const u16* q = (const u16*)p.q + (int64_t)bidb * p.q_batch + (int64_t)t * p.q_row +
                        (int64_t)(kvh * p.group + rg - t * p.group) * p.q_head;
-        auto four = [&](const u16* row) { return in ? *(const u32x2_t*)(row + ch * 4) : u32x2_t{0u, 0u}; };
+        auto four = [&](const u16* row) { return in ? *(const u32x2_t*)(row + col) : u32x2_t{0u, 0u}; };
         auto elt = [](u32x2_t x, int e) { return E::to_f32((u16)(x[e >> 1] >> (e & 1) * 16)); };
-        auto of_row = [&](bool x) { return __ballot(x) >> (lane & ~(CH - 1)) & (~0ull >> (64 - CH)); };
+        const int ln = opaque(lane);
+        auto of_row = [&](bool x) { return __ballot(x) >> (ln & ~(CH - 1)) & (~0ull >> (64 - CH)); };
         const u32x2_t qx = four(q);
         const int last = min(p.mask == nullptr ? min(total, len + t + 1) : total, s1 * kStep);
-        for (int j = max(max(len, split), s0 * kStep); j < last; ++j) {
+        for (int j = max(first_hidden(p, len, mt), s0 * kStep); j < last; ++j) {
           if (!sees(t, j, mask_byte(t, j))) continue;
           bool out = false;
           const int64_t off = has_new ? 0 : slot_offset(c, bidb, j, out);
@@ -496,8 +503,8 @@ __global__ void __launch_bounds__(256, groups_per_cu(D, WM)) kv_attn_kernel(cons
           float dot = 0.f;
 #pragma unroll
           for (int e = 0; e < 4; ++e) dot += elt(qx, e) * elt(k, e);
-#pragma unroll
-          for (int x = 1; x < CH; x <<= 1) dot += __shfl_xor(dot, x);
+#pragma unroll 1
+          for (int x = 1; x < CH; x <<= 1) dot += __shfl_xor(dot, opaque(x));
           const float weight = fast_exp2(fmaf(dot, cs, -lse2));
           bool done = true;                        // (NaN already: no key changes that)
 #pragma unroll
