@@ -278,12 +278,15 @@ __global__ void __launch_bounds__(256, groups_per_cu(D, WM)) kv_attn_kernel(cons
         for (int i = 0; i < St::NI; ++i) {
           const int off = panel_off(St::row(i, ln), St::chunk(ln), NR);
           const unsigned keep = chunk_ok && j0 + St::row(i, ln) < total ? ~0u : 0u;
+          // (cached keys' values may take the path below, too, where it changes nothing for them.  Asking first: tree
+          // of 48 over 16 x 8k keys 148 us, 157 without; at d = 256 it spills: decoding 8 x 26k keys 617, 441 without)
+          const unsigned drafted = D == 256 || j0 + St::row(i, ln) >= len ? ~0u : 0u;
           u32x4_t kx, vx;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             kx[e] = st.k[i][e] & keep;
             vx[e] = st.v[i][e] & keep;
-            odd |= odd_pair<BF16>(vx[e]);
+            odd |= odd_pair<BF16>(vx[e]) & drafted;
           }
           *(u32x4_t*)(mine + off) = kx;
           *(u32x4_t*)(mine + TILE + off) = vx;
