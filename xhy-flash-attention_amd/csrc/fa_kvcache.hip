@@ -34,12 +34,12 @@
 // Keys past a sequence's end load as zeros, so no slot behind it reaches a result.  A sequence whose
 // length does not leave room for the drafted tokens, or that names a page outside the cache, gives NaN.
 //
-// Measured, 32 / 8 heads of 128: 8 sequences of 20k to 32k keys with weights 202 + 14 us (4.4 TB/s of K and V; a
-// step's hand-over through LDS and its products keep a workgroup from more); 4k keys of one sequence 12 + 4 us
-// (latency: one key takes 11.3, by three reads of the lengths, Q, the keys, LDS and the merge one after another); 48
-// drafted tokens over 16 sequences of up to 8k keys in pages of 64: 171 + 13 us under the profiler, 147 in all
+// Measured, 32 / 8 heads of 128: 8 sequences of 20k to 32k keys with weights 201 + 13 us (4.5 TB/s of K and V; a
+// step's hand-over through LDS and its products keep a workgroup from more); 4k keys of one sequence 13 + 4 us
+// (latency: one key takes 11.8, by three reads of the lengths, Q, the keys, LDS and the merge one after another); 48
+// drafted tokens over 16 sequences of up to 8k keys in pages of 64: 164 + 12 us under the profiler, 146 in all
 // without it (softmax and products of 96-row tiles: the fourth wave stages keys only).  A prompt is slow here: 8192
-// tokens 20.7 ms, against 0.42 of the causal forward (all keys for every row tile, and one share is one XCD).
+// tokens 20.5 ms, against 0.42 of the causal forward (all keys for every row tile, and one share is one XCD).
 #include <algorithm>
 #include <stdexcept>
 #include <string>
