@@ -46,10 +46,11 @@ class QKNormRotary(torch.nn.Module):
     """The weights of ``apply_qk_norm_rotary_func`` and, with rotary_dim > 0, its cos / sin table.
 
     The table is fp32, computed in fp64 (angles of far positions keep their digits) for as many rows
-    as asked for, and grows by doubling (the host then waits for it: any stream may use it next); XPos scaling is not part of it.  Tables that were outgrown
-    are kept (all of them together are smaller than the last one): graphs captured with them read them
-    at every replay.  A call in a capture that needs a longer table fills one of its own at every
-    replay; call ``table(rows, device)``, or the step itself, before the capture."""
+    as asked for, and grows by doubling (the host then waits for it: any stream may use it next); XPos
+    scaling is not part of it.  Tables that were outgrown are kept (all of them together are smaller than
+    the last one): graphs captured with them read them at every replay.  A call in a capture that needs a
+    longer table fills one of its own at every replay; call ``table(rows, device)``, or the step itself,
+    before the capture."""
 
     def __init__(self, headdim: int, rotary_dim: int = 0, base: float = 10000.0, interleaved: bool = False,
                  eps: float = 1e-6, device=None, dtype=None):
@@ -75,10 +76,11 @@ class QKNormRotary(torch.nn.Module):
                                     / self.rotary_dim)
                 angle = torch.outer(torch.arange(max(rows, 2 * have), device=device, dtype=torch.float64), inv)
                 made = angle.cos().float(), angle.sin().float()
-            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
-                return made                        # filled by the replays, in the graph's memory: for this call alone
             if device.type == "cuda":
-                torch.cuda.current_stream(device).synchronize()   # whole for calls on other streams
+                with torch.cuda.device(device):
+                    if torch.cuda.is_current_stream_capturing():
+                        return made                # filled by the replays, in the graph's memory: for this call alone
+                    torch.cuda.current_stream().synchronize()   # whole for calls on other streams
             tables.append(made)
         return tables[-1]
 
